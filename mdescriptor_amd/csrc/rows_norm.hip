@@ -193,17 +193,19 @@ __global__ __launch_bounds__(Lanes > 256 ? Lanes : 256, 4) void k_norm_back(cons
     }
     int turn = 0;
     for (int64_t base = int64_t(blockIdx.x) * kRows; base < a.rows; base += int64_t(gridDim.x) * kRows) {
-        // lanes without a row take the last one along for the barrier, and nothing of it: its u is zero
-        const bool there = base + mine < a.rows;
+        // lanes without a row stay for the barrier and load zeros: another row's elements would not cancel (an infinite
+        // gradient times a u of zero is NaN), and its owner may already store grad_x over them
+        const bool there = kRows == 1 || base + mine < a.rows;
         const int64_t row = there ? base + mine : a.rows - 1;
+        const int here = there ? width : 0;
         float t[Units][kUnit], h[Units][kUnit];
         const float rstd = there ? a.rstd[row] : 0.0f;
         float along = 0.0f;
 #pragma unroll
         for (int u = 0; u < Units; ++u) {
             const int col = (lane + u * Lanes) * kUnit;
-            load_unit_together(static_cast<const T*>(a.t) + row * a.t_pitch, col, width, t[u]);
-            load_unit_together(static_cast<const T*>(a.grad) + row * a.grad_pitch, col, width, h[u]);
+            load_unit_together(static_cast<const T*>(a.t) + row * a.t_pitch, col, here, t[u]);
+            load_unit_together(static_cast<const T*>(a.grad) + row * a.grad_pitch, col, here, h[u]);
         }
 #pragma unroll
         for (int u = 0; u < Units; ++u) {
