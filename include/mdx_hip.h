@@ -344,7 +344,8 @@ void mdx_hip_host_free(void* ptr);
  * the default stream) and allocates nothing, so it can be captured into a
  * graph and calls on different streams do not wait for each other.  Calls
  * keep nothing: a workspace is the caller's and is free again when the
- * stream has passed the call.  Errors: mdx_hip_last_error(NULL), per thread.
+ * stream has passed the call.  A workspace of sizes that the call refuses has
+ * zero bytes.  Errors: mdx_hip_last_error(NULL), per thread.
  *
  * Matrices are row-major with a pitch in elements; any pitch >= width and any
  * alignment to the element's own size is taken, 16-byte aligned rows are the

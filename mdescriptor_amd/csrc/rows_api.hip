@@ -30,8 +30,13 @@ struct OnDevice {
 
 constexpr int64_t kMostRows = int64_t(1) << 31; // one workgroup per row at most, in a grid of fewer than 2^31
 constexpr int64_t kMostWidth = int64_t(1) << 31;
+constexpr int64_t kMostResults = int64_t(1) << 39; // of a product: tiles in one grid
 
 int64_t element_size(int32_t dtype) { return dtype == MDX_FLOAT32 ? 4 : dtype == MDX_FLOAT8 ? 1 : 2; }
+
+bool in_range(int64_t rows, int64_t width) {
+    return rows >= 0 && width >= 0 && rows < kMostRows && width < kMostWidth;
+}
 
 void check_shape(int64_t rows, int64_t width) {
     require(rows >= 0 && width >= 0, "rows and width must not be negative");
@@ -83,7 +88,7 @@ int mdx_hip_rms_norm(int device, const mdx_norm_args* args, void* stream) {
 }
 
 int64_t mdx_hip_rms_norm_backward_workspace(int64_t rows, int64_t width) {
-    return mdx::rms_norm_backward_workspace(rows, width);
+    return in_range(rows, width) ? mdx::rms_norm_backward_workspace(rows, width) : 0;
 }
 
 int mdx_hip_rms_norm_backward(int device, const mdx_norm_backward_args* args, void* stream) {
@@ -128,7 +133,8 @@ int mdx_hip_quantize_fp8(int device, const mdx_quantize_args* args, void* stream
 }
 
 int64_t mdx_hip_matmul_fp8_workspace(const mdx_matmul_args* args) {
-    return args == nullptr ? 0 : mdx::matmul_fp8_workspace(*args);
+    if (args == nullptr || !in_range(args->m, args->n) || !in_range(args->k, 0)) return 0;
+    return args->m * args->n < kMostResults ? mdx::matmul_fp8_workspace(*args) : 0;
 }
 
 int mdx_hip_matmul_fp8(int device, const mdx_matmul_args* args, void* stream) {
@@ -139,7 +145,7 @@ int mdx_hip_matmul_fp8(int device, const mdx_matmul_args* args, void* stream) {
         check_shape(g.k, 0);
         check_dtype(g.out_dtype);
         require(g.b_tile == 1 || g.b_tile == 128, "b_tile must be 1 or 128");
-        require(g.m * g.n < int64_t(1) << 39, "the result must have fewer than 2^39 elements"); // tiles in one grid
+        require(g.m * g.n < kMostResults, "the result must have fewer than 2^39 elements");
         if (g.m == 0 || g.n == 0) return;
         check_matrix(g.out, g.out_pitch, g.n, g.out_dtype, "out");
         const int64_t blocks = (g.k + 127) / 128;

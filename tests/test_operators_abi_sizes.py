@@ -1,0 +1,59 @@
+"""Sizes at the limits of the operators' C entry points, without a GPU: every call here is refused, or has nothing to do,
+before a device is touched."""
+
+from __future__ import annotations
+
+import ctypes
+import subprocess
+import sys
+
+import pytest
+
+from conftest import ROOT
+
+pytest.importorskip("torch")
+
+P = 4096  # an address that nothing here reads
+
+
+@pytest.fixture(scope="module")
+def hip():
+    from mdescriptor_amd import _hip
+
+    if not _hip.LIBRARY_PATH.is_file():
+        subprocess.run([sys.executable, "-m", "mdescriptor_amd.build"], check=True, cwd=ROOT)
+    return _hip
+
+
+def matmul(hip, **changes):
+    values = dict(m=40, n=8, k=200, a=P, a_pitch=256, a_scales=P, a_scales_pitch=4, b=P, b_pitch=256, b_scales=P,
+                  b_scales_pitch=4, out=P, out_pitch=8, b_tile=1, out_dtype=1, a_packed=1, b_packed=1)
+    return hip.MatmulArgs(**{**values, **changes})
+
+
+WORKSPACES = """
+import ctypes, sys
+sys.path.insert(0, {root!r})
+from mdescriptor_amd import _hip
+lib = _hip.load_library()
+for sizes in ({{"k": -1}}, {{"k": -63}}, {{"k": -64}}, {{"k": -200}}, {{"m": -40}}, {{"n": -8}}, {{"k": 1 << 31}},
+              {{"k": 1 << 62}}, {{"m": 1 << 62, "n": 1 << 62}}, {{"m": (1 << 31) - 1, "n": (1 << 31) - 1}}):
+    args = _hip.MatmulArgs(**{{**dict(m=40, n=8, k=200, out_dtype=1, b_tile=1), **sizes}})
+    assert lib.mdx_hip_matmul_fp8_workspace(ctypes.byref(args)) == 0, sizes
+for rows, width in ((-1, 5), (5, -1), (1 << 31, 5), (5, 1 << 31), (1 << 62, 1 << 62)):
+    assert lib.mdx_hip_rms_norm_backward_workspace(rows, width) == 0, (rows, width)
+"""
+
+
+def test_workspaces_of_refused_sizes_are_empty():
+    """In a process of its own: sizes that a workspace's arithmetic does not expect must not end the caller."""
+
+    done = subprocess.run([sys.executable, "-c", WORKSPACES.format(root=str(ROOT))], capture_output=True, text=True)
+    assert done.returncode == 0, done.stderr
+
+
+def test_workspaces_of_taken_sizes_hold_their_parts(hip):
+    lib = hip.load_library()
+    size = lib.mdx_hip_matmul_fp8_workspace(ctypes.byref(matmul(hip, a_packed=0)))
+    assert size >= 40 * 256 + 40 * 2 and size % 16 == 0
+    assert lib.mdx_hip_rms_norm_backward_workspace(1000, 256) >= 256 * 4
