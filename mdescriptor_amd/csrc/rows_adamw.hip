@@ -23,6 +23,7 @@ typedef uint32_t u2_any __attribute__((ext_vector_type(2), aligned(1))); // eigh
 
 constexpr int kTensors = 48;            // per launch: 48 * 72 bytes of arguments, under the 4 KB of a launch
 constexpr int kChunk = 256 * kUnit;    // elements per workgroup: with two or four units a lane, 5 and 20 % slower
+static_assert(kChunk == kAdamwChunk, "the size that the entry point refuses follows from it");
 
 struct AdamwTable {
     float* params[kTensors];
@@ -175,7 +176,7 @@ void adamw_step(const mdx_adamw_args& g, hipStream_t s) {
     t.rest1 = float(1.0 - g.beta1);
     t.rest2 = float(1.0 - g.beta2);
     t.seed = g.seed;
-    constexpr int64_t kMostChunks = 1 << 30; // workgroups per launch
+    constexpr int64_t kMostChunks = kAdamwMost / kChunk; // workgroups per launch
     auto flush = [&] {
         if (t.count == 0) return;
         const bool codes = g.bits == 8;

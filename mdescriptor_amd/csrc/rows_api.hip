@@ -28,9 +28,9 @@ struct OnDevice {
     }
 };
 
-constexpr int64_t kMostRows = int64_t(1) << 31; // one workgroup per row at most, in a grid of fewer than 2^31
+constexpr int64_t kMostRows = int64_t(1) << 31; // with widths below 2^31 too, products of two sizes fit 64 bits
 constexpr int64_t kMostWidth = int64_t(1) << 31;
-constexpr int64_t kMostResults = int64_t(1) << 39; // of a product: tiles in one grid
+constexpr int64_t kMostResults = int64_t(1) << 39; // of a product, so that its bytes do too
 
 int64_t element_size(int32_t dtype) { return dtype == MDX_FLOAT32 ? 4 : dtype == MDX_FLOAT8 ? 1 : 2; }
 
@@ -188,7 +188,7 @@ int mdx_hip_adamw_step(int device, const mdx_adamw_args* args, void* stream) {
         require(std::isfinite(g.weight_decay) && g.weight_decay >= 0.0, "weight_decay must be finite and not negative");
         for (int64_t i = 0; i < g.count; ++i) {
             const mdx_adamw_tensor& x = g.tensors[i];
-            require(x.n >= 0 && x.n < (int64_t(1) << 42), "a tensor's size must lie in [0, 2^42)");
+            require(x.n >= 0 && x.n <= mdx::kAdamwMost, "a tensor's size must lie in [0, 2^35 - 2^11]");
             if (x.n == 0) continue;
             check_matrix(x.params, x.n, x.n, MDX_FLOAT32, "params");
             check_matrix(x.grads, x.n, x.n, g.grad_dtype, "grads");

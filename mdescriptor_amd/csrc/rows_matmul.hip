@@ -128,13 +128,13 @@ __device__ __forceinline__ i8 load_block(const uint8_t* block, int quarter, int6
 // 1,024 x 3,696: 4.8 us).  From 17 rows on tiles read b once for more of them (64
 // x 4,096 x 7,380: 12.5 us).
 template <typename O, int MT, int NT, int Waves>
-__global__ __launch_bounds__(Waves * kWave) void k_matmul_few(const MatmulView a, int64_t tiles_n) {
+__global__ __launch_bounds__(Waves * kWave) void k_matmul_few(const MatmulView a, int64_t tiles_n, int64_t first) {
     constexpr bool kExact = sizeof(O) == 4;
     __shared__ f4 join[Waves > 1 ? Waves - 1 : 1][MT * NT][kWave];
     const int lane = threadIdx.x % kWave, r = lane % 16, quarter = lane / 16;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int64_t tile_m = int64_t(blockIdx.x) / tiles_n;
-    const int64_t m0 = tile_m * 16 * MT, n0 = (int64_t(blockIdx.x) - tile_m * tiles_n) * 16 * NT;
+    const int64_t at = first + int64_t(blockIdx.x), tile_m = at / tiles_n;
+    const int64_t m0 = tile_m * 16 * MT, n0 = (at - tile_m * tiles_n) * 16 * NT;
     const int64_t blocks = (a.k + kScaleBlock - 1) / kScaleBlock;
     const uint8_t *rows_a[MT], *rows_b[NT], *scales_a[MT], *scales_b[NT];
 #pragma unroll
@@ -541,9 +541,9 @@ __global__ __launch_bounds__(WR * WC * kWave) void k_matmul_tile(const MatmulVie
 // An operand whose rows are not aligned, copied to rows that are: 16 bytes a
 // lane, zeros past the width.
 __global__ __launch_bounds__(256) void k_pack(const uint8_t* from, int64_t pitch, int64_t rows, int64_t width,
-                                              uint8_t* to, int64_t to_pitch) {
+                                              uint8_t* to, int64_t to_pitch, int64_t first) {
     const int64_t pieces = to_pitch / 16;
-    const int64_t at = int64_t(blockIdx.x) * 256 + threadIdx.x;
+    const int64_t at = (first + int64_t(blockIdx.x)) * 256 + threadIdx.x;
     if (at >= rows * pieces) return;
     const int64_t row = at / pieces, col = (at - row * pieces) * 16;
     u4 w{0u, 0u, 0u, 0u};
@@ -630,25 +630,27 @@ struct Packed {
 void pack(const uint8_t* from, int64_t pitch, int64_t rows, int64_t width, uint8_t* to, int64_t to_pitch,
           hipStream_t s) {
     const int64_t pieces = rows * (to_pitch / 16);
-    k_pack<<<dim3(unsigned((pieces + 255) / 256)), 256, 0, s>>>(from, pitch, rows, width, to, to_pitch);
-    MDX_HIP(hipGetLastError());
+    in_runs((pieces + 255) / 256, 256, [&](int64_t first, int64_t count) {
+        k_pack<<<dim3(unsigned(count)), 256, 0, s>>>(from, pitch, rows, width, to, to_pitch, first);
+        MDX_HIP(hipGetLastError());
+    });
 }
 
 // ------------------------------------------------------------ which kernel
 
-// Rows and columns of a tile, workgroups of it that a CU holds, and what a
+// Rows and columns of a tile, its lanes, workgroups of it that a CU holds, and what a
 // stage of 64 takes: microseconds when a workgroup is alone on its CU (waiting
 // for memory and barriers) and per workgroup when a CU is full, and what a tile
 // takes beside its stages.  Measured on the products of 8,192^3, 2,000 x 1,500 x
 // 2,500 and 300 x 500 x 3,000 for 16-bit and float32 results.
 struct TileCost {
-    int rows, cols, held;
+    int rows, cols, lanes, held;
     double alone[2], full[2], fixed;
 };
 constexpr TileCost kTiles[3] = {
-    {256, 256, 1, {0.66, 1.62}, {0.66, 1.62}, 7.0},
-    {128, 128, 2, {0.25, 0.52}, {0.34, 0.46}, 2.5},
-    {64, 64, 4, {0.13, 0.20}, {0.163, 0.19}, 1.5},
+    {256, 256, 512, 1, {0.66, 1.62}, {0.66, 1.62}, 7.0},
+    {128, 128, 256, 2, {0.25, 0.52}, {0.34, 0.46}, 2.5},
+    {64, 64, 256, 4, {0.13, 0.20}, {0.163, 0.19}, 1.5},
 };
 constexpr int64_t kUnits = 256;     // CUs of the device
 constexpr double kJoin = 4.5;       // microseconds of the second launch where the contraction is split
@@ -677,7 +679,7 @@ MatmulPlan plan_matmul(const mdx_matmul_args& g) {
     for (int t = 0; t < 3; ++t) {
         const TileCost& c = kTiles[t];
         const int64_t tiles = ((g.m + c.rows - 1) / c.rows) * ((g.n + c.cols - 1) / c.cols);
-        if (tiles >= (int64_t(1) << 28)) continue;
+        if ((tiles + 7) / 8 * 8 * c.lanes >= int64_t(1) << 32) continue; // one launch
         for (int64_t asked = 1; asked <= 64; asked = asked < 4 ? asked + 1 : asked * 5 / 4) {
             const int64_t per = asked == 1 ? stages : ((stages + asked - 1) / asked + 7) / 8 * 8;
             const int64_t slices = (stages + per - 1) / per; // fewer than asked for, where whole dwords of scales end early
@@ -718,8 +720,10 @@ template <typename O> void run_matmul(const MatmulView& v, const MatmulPlan& pla
     constexpr bool kExact = sizeof(O) == 4;
     if (plan.tile < 0) {
         const int64_t tiles_n = (v.n + 15) / 16, tiles_m = (v.m + 15) / 16;
-        k_matmul_few<O, 1, 1, 8><<<dim3(unsigned(tiles_m * tiles_n)), 512, 0, s>>>(v, tiles_n);
-        MDX_HIP(hipGetLastError());
+        in_runs(tiles_m * tiles_n, 512, [&](int64_t first, int64_t count) {
+            k_matmul_few<O, 1, 1, 8><<<dim3(unsigned(count)), 512, 0, s>>>(v, tiles_n, first);
+            MDX_HIP(hipGetLastError());
+        });
     } else if (plan.slices == 1) {
         run_tiles<O, kExact>(v, plan, s);
     } else {

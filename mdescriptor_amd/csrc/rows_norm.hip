@@ -136,12 +136,30 @@ __global__ __launch_bounds__(Lanes > 256 ? Lanes : 256) void k_norm(const NormVi
     }
 }
 
+// Rows first..first+most-1, as far as there are such.
+template <typename T, bool Codes> NormView rows_from(NormView a, int64_t first, int64_t most) {
+    a.rows = std::min(a.rows - first, most);
+    a.x = static_cast<const T*>(a.x) + first * a.x_pitch;
+    if (a.residual != nullptr) a.residual = static_cast<const T*>(a.residual) + first * a.residual_pitch;
+    if (a.total != nullptr) a.total = static_cast<T*>(a.total) + first * a.total_pitch;
+    if (a.rstd != nullptr) a.rstd += first;
+    if constexpr (Codes) {
+        a.values = static_cast<uint8_t*>(a.values) + first * a.values_pitch;
+        a.scales += first * a.scales_pitch;
+    } else {
+        a.values = static_cast<T*>(a.values) + first * a.values_pitch;
+    }
+    return a;
+}
+
 template <typename T, bool Codes, int Lanes, int Units> void launch_norm(const NormView& a, bool past, hipStream_t s) {
     constexpr int kThreads = Lanes > 256 ? Lanes : 256, kRows = kThreads / Lanes;
-    const dim3 groups(unsigned((a.rows + kRows - 1) / kRows));
-    if (past) k_norm<T, Codes, Lanes, Units, true><<<groups, kThreads, 0, s>>>(a);
-    else k_norm<T, Codes, Lanes, Units, false><<<groups, kThreads, 0, s>>>(a);
-    MDX_HIP(hipGetLastError());
+    in_runs((a.rows + kRows - 1) / kRows, kThreads, [&](int64_t first, int64_t count) {
+        const NormView b = rows_from<T, Codes>(a, first * kRows, count * kRows);
+        if (past) k_norm<T, Codes, Lanes, Units, true><<<dim3(unsigned(count)), kThreads, 0, s>>>(b);
+        else k_norm<T, Codes, Lanes, Units, false><<<dim3(unsigned(count)), kThreads, 0, s>>>(b);
+        MDX_HIP(hipGetLastError());
+    });
 }
 
 template <typename T, bool Codes> void choose_norm(const NormView& a, bool past, hipStream_t s) {
@@ -319,11 +337,12 @@ template <typename T> __global__ __launch_bounds__(256) void k_norm_gain_long(co
 // Sum of the workgroups' partial rows: Cols columns per workgroup, 1024 / Cols
 // groups of rows side by side, joined pairwise.
 template <int Cols>
-__global__ __launch_bounds__(1024) void k_norm_gain(const float* part, int64_t parts, int64_t width, float* out) {
+__global__ __launch_bounds__(1024) void k_norm_gain(const float* part, int64_t parts, int64_t width, float* out,
+                                                    int64_t first) {
     constexpr int kGroups = 1024 / Cols;
     __shared__ float sums[kGroups][Cols + 1];
     const int mine = threadIdx.x % Cols, group = threadIdx.x / Cols;
-    const int64_t col = int64_t(blockIdx.x) * Cols + mine;
+    const int64_t col = (first + int64_t(blockIdx.x)) * Cols + mine;
     float s = 0.0f;
     if (col < width) {
         int64_t p = group;
@@ -392,8 +411,25 @@ template <typename T> void choose_back(const BackView& a, const BackShape& b, hi
     const dim3 strips(unsigned((a.width + 2047) / 2048), unsigned(b.groups));
     k_norm_gain_long<T><<<strips, 256, 0, s>>>(a);
     MDX_HIP(hipGetLastError());
-    k_norm_back_long<T><<<dim3(unsigned(a.rows)), 1024, 0, s>>>(a);
-    MDX_HIP(hipGetLastError());
+    in_runs(a.rows, 1024, [&](int64_t first, int64_t count) {
+        BackView part = a;
+        part.rows = count;
+        part.grad = static_cast<const T*>(a.grad) + first * a.grad_pitch;
+        part.t = static_cast<const T*>(a.t) + first * a.t_pitch;
+        if (a.grad_total != nullptr) part.grad_total = static_cast<const T*>(a.grad_total) + first * a.grad_total_pitch;
+        part.rstd = a.rstd + first;
+        part.grad_x = static_cast<T*>(a.grad_x) + first * a.grad_x_pitch;
+        k_norm_back_long<T><<<dim3(unsigned(count)), 1024, 0, s>>>(part);
+        MDX_HIP(hipGetLastError());
+    });
+}
+
+template <int Cols>
+void launch_gain(const float* part, int64_t parts, int64_t width, float* out, hipStream_t s) {
+    in_runs((width + Cols - 1) / Cols, 1024, [&](int64_t first, int64_t count) {
+        k_norm_gain<Cols><<<dim3(unsigned(count)), 1024, 0, s>>>(part, parts, width, out, first);
+        MDX_HIP(hipGetLastError());
+    });
 }
 
 } // namespace
@@ -431,9 +467,8 @@ void rms_norm_backward(const mdx_norm_backward_args& g, hipStream_t s) {
     // a sum over no rows is zero
     const int64_t parts = g.rows > 0 ? b.groups : 0;
     // few columns: more workgroups of fewer (50,225 x 176 bfloat16, both launches: 16.9 us, 17.7 with 32 columns each)
-    if (g.width <= 512) k_norm_gain<8><<<dim3(unsigned((g.width + 7) / 8)), 1024, 0, s>>>(a.part, parts, g.width, g.grad_gain);
-    else k_norm_gain<32><<<dim3(unsigned((g.width + 31) / 32)), 1024, 0, s>>>(a.part, parts, g.width, g.grad_gain);
-    MDX_HIP(hipGetLastError());
+    if (g.width <= 512) launch_gain<8>(a.part, parts, g.width, g.grad_gain, s);
+    else launch_gain<32>(a.part, parts, g.width, g.grad_gain, s);
 }
 
 } // namespace mdx

@@ -28,8 +28,8 @@ struct QuantizeView {
 };
 
 // One scale per row and block: sixteen lanes a block, one unit a lane.
-template <typename T> __global__ __launch_bounds__(256) void k_quantize_rows(const QuantizeView a, int64_t blocks) {
-    const int64_t at = (int64_t(blockIdx.x) * 256 + threadIdx.x) / 16;
+template <typename T> __global__ __launch_bounds__(256) void k_quantize_rows(const QuantizeView a, int64_t blocks, int64_t first) {
+    const int64_t at = ((first + int64_t(blockIdx.x)) * 256 + threadIdx.x) / 16;
     if (at >= a.rows * blocks) return;
     const int64_t row = at / blocks, block = at - row * blocks;
     const int64_t col = block * kScaleBlock + (threadIdx.x % 16) * kUnit;
@@ -143,8 +143,10 @@ __global__ __launch_bounds__(16 * kScaleBlock / Rows) void k_quantize_tile(const
 template <typename T> void choose_quantize(const QuantizeView& a, bool whole, bool turned, hipStream_t s) {
     const int64_t across = (a.width + kScaleBlock - 1) / kScaleBlock, down = (a.rows + kScaleBlock - 1) / kScaleBlock;
     if (!whole && !turned) {
-        k_quantize_rows<T><<<dim3(unsigned((a.rows * across + 15) / 16)), 256, 0, s>>>(a, across);
-        MDX_HIP(hipGetLastError());
+        in_runs((a.rows * across + 15) / 16, 256, [&](int64_t first, int64_t count) {
+            k_quantize_rows<T><<<dim3(unsigned(count)), 256, 0, s>>>(a, across, first);
+            MDX_HIP(hipGetLastError());
+        });
         return;
     }
     constexpr int64_t kMostDown = 32768; // tiles in the grid's second dimension
@@ -155,12 +157,20 @@ template <typename T> void choose_quantize(const QuantizeView& a, bool whole, bo
         b.rows = std::min<int64_t>(a.rows - skip, kMostDown * kScaleBlock);
         b.codes = a.codes + (turned ? skip : skip * a.codes_pitch);
         b.scales = a.scales + (turned ? first : (whole ? first : skip) * a.scales_pitch);
-        const dim3 grid(unsigned(across), unsigned((b.rows + kScaleBlock - 1) / kScaleBlock));
-        // many lanes a tile: 1,024 x 3,696 has fewer tiles than the device CUs (whole tiles 4.6 us, 7.0 with 256 lanes)
-        if (whole && turned) k_quantize_tile<T, true, true, 4><<<grid, 512, 0, s>>>(b);
-        else if (whole) k_quantize_tile<T, true, false, 2><<<grid, 1024, 0, s>>>(b);
-        else k_quantize_tile<T, false, true, 4><<<grid, 512, 0, s>>>(b);
-        MDX_HIP(hipGetLastError());
+        in_runs(across, 1024, [&](int64_t left, int64_t count) {
+            QuantizeView c = b;
+            const int64_t over = left * kScaleBlock;
+            c.x = static_cast<const T*>(b.x) + over;
+            c.width = std::min<int64_t>(b.width - over, count * kScaleBlock);
+            c.codes = b.codes + (turned ? over * b.codes_pitch : over);
+            c.scales = b.scales + (turned ? (whole ? left : over) * b.scales_pitch : left);
+            const dim3 grid(unsigned(count), unsigned((b.rows + kScaleBlock - 1) / kScaleBlock));
+            // many lanes a tile: 1,024 x 3,696 has fewer tiles than the device CUs (whole tiles 4.6 us, 7.0 with 256 lanes)
+            if (whole && turned) k_quantize_tile<T, true, true, 4><<<grid, 512, 0, s>>>(c);
+            else if (whole) k_quantize_tile<T, true, false, 2><<<grid, 1024, 0, s>>>(c);
+            else k_quantize_tile<T, false, true, 4><<<grid, 512, 0, s>>>(c);
+            MDX_HIP(hipGetLastError());
+        });
     }
 }
 

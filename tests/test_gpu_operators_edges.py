@@ -123,3 +123,118 @@ def test_norm_whose_total_is_an_input(dtype, shape, to_codes):
         assert torch.equal(values.float(), want.values.float())
         if to_codes:
             assert torch.equal(scales, want.scales.contiguous().view(torch.uint8))
+
+
+# ------------------------------------------ sizes past one launch's lanes
+
+# A launch takes 2^28 lanes: what needs more goes in several.  The whole has to be what calls on its parts give.
+
+
+@pytest.fixture
+def freed():
+    yield
+    torch.cuda.empty_cache()
+
+
+def by_parts(x, at, call):
+    return torch.cat([call(x[:at]), call(x[at:])])
+
+
+def raw(x: torch.Tensor) -> torch.Tensor:
+    return x.contiguous().view(torch.uint8) if x.element_size() == 1 else x
+
+
+def test_norm_of_more_rows_than_a_launch_takes(freed):
+    rows = (1 << 24) + 37  # sixteen lanes each
+    x, r, gain = randn(20, rows, 1, dtype=torch.bfloat16), randn(21, rows, 1, dtype=torch.bfloat16), randn(22, 1)
+    got = mdx.rms_norm(x, gain, residual=r)
+    at = 1 << 23
+    parts = [mdx.rms_norm(x[part], gain, residual=r[part]) for part in (slice(0, at), slice(at, None))]
+    for name in ("values", "total", "rstd"):
+        assert torch.equal(getattr(got, name), torch.cat([getattr(p, name) for p in parts]))
+    codes = mdx.rms_norm(x, gain, dtype=CODES)
+    for name in ("values", "scales"):
+        assert torch.equal(raw(getattr(codes, name)),
+                           by_parts(x, at, lambda p: raw(getattr(mdx.rms_norm(p, gain, dtype=CODES), name))))
+
+
+def test_gradients_of_more_wide_rows_than_a_launch_takes(freed):
+    rows, width = (1 << 18) + 3, 16385  # a workgroup of 1,024 lanes each
+    g = torch.Generator(device="cuda").manual_seed(23)
+    t, grad = (torch.randn(rows, width, generator=g, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    gain, rstd = randn(24, width), randn(25, rows).abs()
+    last = mdx.rms_norm_backward(grad[-5:], t[-5:], gain, rstd[-5:], grad_total=grad[-5:])[0]
+    grad_gain = backward_into(grad, t, gain, rstd, grad, grad)
+    assert torch.equal(grad[-5:], last) and torch.isfinite(grad_gain).all()
+
+
+def test_gradient_of_a_gain_of_more_columns_than_a_launch_takes(freed):
+    width = (1 << 23) + 77  # 1,024 lanes for 32 columns
+    t, grad, gain, rstd = randn(26, 2, width), randn(27, 2, width), randn(28, width), randn(29, 2).abs()
+    got = mdx.rms_norm_backward(grad, t, gain, rstd)[1]
+    terms = grad.double() * (t.double() * rstd.double()[:, None])
+    assert torch.all((got.double() - terms.sum(dim=0)).abs() <= 10 * U * terms.abs().sum(dim=0))
+    assert not mdx.rms_norm_backward(grad[:0], t[:0], gain, rstd[:0])[1].any()
+
+
+def test_quantize_of_more_blocks_than_a_launch_takes(freed):
+    x = randn(30, (1 << 24) + 37, 1, dtype=torch.float16)  # sixteen lanes a block
+    codes, scales = mdx.quantize_fp8(x)
+    for which, whole in enumerate((codes, scales)):
+        assert torch.equal(raw(whole), by_parts(x, 1 << 23, lambda p: raw(mdx.quantize_fp8(p)[which])))
+
+
+@pytest.mark.parametrize("tile, transpose", [(128, False), (128, True), (1, True)])
+@pytest.mark.parametrize("shape", [(3, (1 << 25) + 130), ((1 << 22) + 1, 1)])
+def test_quantize_of_more_tiles_than_a_launch_takes(freed, tile, transpose, shape):
+    """Across (2^18 tiles a launch) and down (32,768)."""
+
+    x = randn(31, *shape, dtype=torch.bfloat16)
+    wide = shape[1] > shape[0]
+    at = 1 << (24 if wide else 21)
+    parts = [mdx.quantize_fp8(p, block=(tile, 128), transpose=transpose)
+             for p in ((x[:, :at], x[:, at:]) if wide else (x[:at], x[at:]))]
+    whole = mdx.quantize_fp8(x, block=(tile, 128), transpose=transpose)
+    for which in range(2):
+        assert torch.equal(raw(whole[which]), torch.cat([raw(p[which]) for p in parts], dim=int(wide != transpose)))
+
+
+def test_product_of_more_columns_than_a_launch_takes(freed):
+    n = (1 << 23) + 40  # 512 lanes for 16 x 16 results
+    g = torch.Generator(device="cuda").manual_seed(32)
+    b, sb = mdx.quantize_fp8(torch.randn(n, 128, generator=g, device="cuda", dtype=torch.bfloat16))
+    a, sa = mdx.quantize_fp8(randn(33, 3, 128))
+    got = mdx.matmul_fp8(a, sa, b, sb)
+    at = 1 << 22
+    assert torch.equal(got, torch.cat([mdx.matmul_fp8(a, sa, b[:at], sb[:at]), mdx.matmul_fp8(a, sa, b[at:], sb[at:])], 1))
+    none = torch.empty(20, 0, dtype=torch.uint8, device="cuda")
+    zeros = mdx.matmul_fp8(none.view(CODES), none.view(SCALES), b[:, :0], sb[:, :0])
+    assert zeros.shape == (20, n) and not zeros.any()
+
+
+def test_product_of_more_unaligned_rows_than_a_launch_packs(freed):
+    n, k = (1 << 25) + 3, 100  # eight pieces of 16 bytes a row
+    g = torch.Generator(device="cuda").manual_seed(34)
+    b = torch.empty(n, k, dtype=torch.uint8, device="cuda")
+    for part in b.split(1 << 22):
+        part.copy_(torch.randint(0, 256, part.shape, generator=g, device="cuda", dtype=torch.uint8) & 0xF7)  # no NaN
+    b, sb = b.view(CODES), torch.randint(120, 130, (n, 1), generator=g, device="cuda", dtype=torch.uint8).view(SCALES)
+    a, sa = mdx.quantize_fp8(randn(35, 1, k))
+    got = mdx.matmul_fp8(a, sa, b, sb)
+    at = 1 << 24
+    assert torch.equal(got, torch.cat([mdx.matmul_fp8(a, sa, b[:at], sb[:at]), mdx.matmul_fp8(a, sa, b[at:], sb[at:])], 1))
+    assert torch.isfinite(got).all() and got.any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_product_of_rows_far_apart(freed, dtype):
+    """Rows of 2^22 bytes and more take the kernel for few rows, at any number of them.  Whole numbers: exact."""
+
+    m, n, k, pitch = 40, 24, 200, 1 << 22
+    g = torch.Generator(device="cuda").manual_seed(36)
+    a, b = (torch.randint(-15, 16, (rows, k), generator=g, device="cuda").float() for rows in (m, n))
+    far = torch.empty(m, pitch, dtype=torch.uint8, device="cuda").view(CODES)[:, :k]
+    far.copy_(a.to(CODES))
+    ones = [torch.full((rows, 2), 127, dtype=torch.uint8, device="cuda").view(SCALES) for rows in (m, n)]
+    got = mdx.matmul_fp8(far, ones[0], b.to(CODES), ones[1], dtype=dtype)
+    assert torch.equal(got, (a.double() @ b.double().T.contiguous()).to(dtype))

@@ -57,3 +57,15 @@ def test_workspaces_of_taken_sizes_hold_their_parts(hip):
     size = lib.mdx_hip_matmul_fp8_workspace(ctypes.byref(matmul(hip, a_packed=0)))
     assert size >= 40 * 256 + 40 * 2 and size % 16 == 0
     assert lib.mdx_hip_rms_norm_backward_workspace(1000, 256) >= 256 * 4
+
+
+def test_adamw_refuses_tensors_of_more_than_one_launch(hip):
+    """256 lanes for 2,048 elements, fewer than 2^32 lanes: the count is checked before anything is queued."""
+
+    lib = hip.load_library()
+    for n in ((1 << 35) - 2047, 1 << 35, 1 << 41):
+        table = (hip.AdamwTensor * 1)(hip.AdamwTensor(n, P, P, P, P, P, P))
+        args = hip.AdamwArgs(tensors=ctypes.addressof(table), count=1, lr=1e-3, beta1=0.9, beta2=0.99, eps=1e-8,
+                             weight_decay=0.0, step=1, seed=0, grad_dtype=1, bits=8)
+        assert lib.mdx_hip_adamw_step(0, ctypes.byref(args), None) == hip.MDX_INVALID_ARGUMENT
+        assert "size" in lib.mdx_hip_last_error(None).decode()
