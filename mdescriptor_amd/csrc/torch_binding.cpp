@@ -130,6 +130,11 @@ at::Tensor empty_scales(int64_t rows, int64_t width, at::Device d) {
     return empty_pitched(rows, ceil_div(width, kBlock), 4, kScales, d);
 }
 
+// Tells autograd that a tensor which the caller gave was written: graphs that saved it refuse to go on.
+void written_to(const at::Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version(); // tensors made in inference mode have no version
+}
+
 void* stream_of(at::Device device) { return c10::hip::getCurrentHIPStream(device.index()).stream(); }
 
 template <typename Call> void run(const char* name, Call&& call) {
@@ -427,6 +432,7 @@ PyObject* matmul_fp8(PyObject*, PyObject* const* o, Py_ssize_t n) {
             }
             void* stream = stream_of(device);
             run("matmul_fp8", [&] { return mdx_hip_matmul_fp8(device.index(), &g, stream); });
+            if (o[5] != Py_None) written_to(out);
         }
         return THPVariable_Wrap(out);
     });
@@ -492,6 +498,8 @@ PyObject* adamw_step(PyObject*, PyObject* const* o, Py_ssize_t n) {
         std::vector<mdx_adamw_tensor> table(static_cast<size_t>(count));
         std::vector<void*> written;
         written.reserve(static_cast<size_t>(count) * 5);
+        std::vector<at::Tensor> moved; // held: the lists are the caller's, and may change while the call lets go of Python
+        moved.reserve(static_cast<size_t>(count) * 5);
         for (Py_ssize_t k = 0; k < count; ++k) {
             void* at_[6] = {};
             const at::Tensor& param = given[0]->at(k);
@@ -510,6 +518,7 @@ PyObject* adamw_step(PyObject*, PyObject* const* o, Py_ssize_t n) {
                     throw Refused{std::string(names[i]) + " must have the shapes of params", names[i]};
                 }
                 at_[i] = t.data_ptr();
+                if (i != 1) moved.push_back(t);
                 if (i != 1 && size > 0) written.push_back(at_[i]);
             }
             table[size_t(k)] = {size, static_cast<float*>(at_[0]), at_[1], at_[2], at_[3],
@@ -522,6 +531,7 @@ PyObject* adamw_step(PyObject*, PyObject* const* o, Py_ssize_t n) {
         a.count = count;
         void* stream = stream_of(device);
         run("adamw_step", [&] { return mdx_hip_adamw_step(device.index(), &a, stream); });
+        for (const at::Tensor& t : moved) written_to(t);
         return none();
     });
 }

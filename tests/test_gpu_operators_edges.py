@@ -238,3 +238,40 @@ def test_product_of_rows_far_apart(freed, dtype):
     ones = [torch.full((rows, 2), 127, dtype=torch.uint8, device="cuda").view(SCALES) for rows in (m, n)]
     got = mdx.matmul_fp8(far, ones[0], b.to(CODES), ones[1], dtype=dtype)
     assert torch.equal(got, (a.double() @ b.double().T.contiguous()).to(dtype))
+
+
+# --------------------------------------------------------------- autograd
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_step_is_seen_by_graphs_that_saved_what_it_writes(bits):
+    """A backward pass through a weight that has moved since must not give gradients of the new weight."""
+
+    weight = randn(40, 300).requires_grad_()
+    loss = weight.square().sum()
+    state = mdx.adamw_state([weight], bits=bits)
+    before = [t._version for part in state if part is not None for t in part]
+    mdx.adamw_step([weight.detach()], [torch.ones(300, device="cuda")], *state, step=1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    assert all(t._version > v for t, v in zip((t for part in state if part is not None for t in part), before))
+    weight.square().sum().backward()  # a new graph is whole again
+    assert torch.equal(weight.grad, 2 * weight.detach())
+
+
+def test_a_product_into_a_buffer_is_seen_by_graphs_that_saved_it():
+    codes, scales = mdx.quantize_fp8(randn(41, 20, 256))
+    out, factor = torch.ones(20, 24, device="cuda"), randn(42, 20, 20).requires_grad_()
+    loss = (out[:, :20] * factor).sum()
+    mdx.matmul_fp8(codes, scales, codes, scales, out=out[:, :20])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+def test_tensors_of_inference_mode_are_written_too():
+    with torch.inference_mode():
+        codes, scales = mdx.quantize_fp8(randn(43, 20, 256))
+        out = torch.zeros(20, 20, device="cuda")
+        mdx.matmul_fp8(codes, scales, codes, scales, out=out)
+        p = torch.zeros(100, device="cuda")
+        mdx.adamw_step([p], [torch.ones(100, device="cuda")], *mdx.adamw_state([p], bits=8), step=1, lr=0.5)
+    assert torch.equal(out, mdx.matmul_fp8(codes, scales, codes, scales, dtype=torch.float32)) and torch.all(p < -0.49)
