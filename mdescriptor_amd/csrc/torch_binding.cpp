@@ -12,12 +12,16 @@
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Dtype.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
 #include <cmath>
 #include <memory>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "../../include/mdx_hip.h"
@@ -135,6 +139,42 @@ void written_to(const at::Tensor& t) {
     if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version(); // tensors made in inference mode have no version
 }
 
+// The calls record no gradients.  Where one would have to go back through a call's results (grad mode is on and an input
+// requires gradients), the results lead to an error in place of nothing: a gradient that is left out of a sum shows nowhere.
+class History {
+public:
+    History(const char* name, std::initializer_list<std::pair<const at::Tensor*, const char*>> inputs) : name_(name) {
+        for (const auto& [t, what] : inputs) {
+            if (!t->defined() || t->unsafeGetTensorImpl()->autograd_meta() == nullptr) continue; // nothing to do with gradients
+            if (t->_fw_grad(0).defined())
+                throw Refused{std::string(what) + " has a forward gradient, and " + name + " gives none", what};
+            if (t->requires_grad() && at::GradMode::is_enabled()) from_.emplace_back(t, what);
+        }
+    }
+    // of an `out` that the caller gave, as for torch's own
+    void refuse_out(const at::Tensor& out) const {
+        if (!from_.empty()) throw Refused{std::string("out records no gradients, but ") + from_[0].second + " requires them", "out"};
+        if (out.requires_grad() && at::GradMode::is_enabled())
+            throw Refused{"out requires gradients: write into it under torch.no_grad()", "out"};
+    }
+    void goes_to(std::initializer_list<at::Tensor> results) const {
+        if (from_.empty()) return;
+        torch::autograd::edge_list edges;
+        for (const auto& [t, what] : from_) edges.push_back(torch::autograd::impl::gradient_edge(*t));
+        const std::shared_ptr<torch::autograd::Node> node(
+            new torch::autograd::NotImplemented(std::string(name_) + " (it records no gradients: call it under torch.no_grad() "
+                                                                     "or in a torch.autograd.Function)",
+                                                std::move(edges)),
+            torch::autograd::deleteNode);
+        for (const at::Tensor& t : results)
+            if (t.defined() && at::isFloatingType(t.scalar_type())) torch::autograd::set_history(t, node);
+    }
+
+private:
+    const char* name_;
+    std::vector<std::pair<const at::Tensor*, const char*>> from_;
+};
+
 void* stream_of(at::Device device) { return c10::hip::getCurrentHIPStream(device.index()).stream(); }
 
 template <typename Call> void run(const char* name, Call&& call) {
@@ -243,6 +283,7 @@ PyObject* rms_norm(PyObject*, PyObject* const* o, Py_ssize_t n) {
             a.residual = residual.data_ptr();
         }
         a.gain = vector_of(o[1], "gain", a.width, device);
+        const History history("rms_norm", {{&rows, "rows"}, {&THPVariable_Unpack(o[1]), "gain"}, {&residual, "residual"}});
         if (a.out_dtype == MDX_FLOAT8) {
             values = empty_codes(a.rows, a.width, device);
             scales = empty_scales(a.rows, a.width, device);
@@ -267,6 +308,7 @@ PyObject* rms_norm(PyObject*, PyObject* const* o, Py_ssize_t n) {
         } else if (a.rows > 0) {
             rstd.fill_(1.0 / std::sqrt(a.eps));
         }
+        history.goes_to({values, scales, total, rstd});
         return tuple_of({values, scales, total, rstd});
     });
 }
@@ -288,14 +330,17 @@ PyObject* rms_norm_backward(PyObject*, PyObject* const* o, Py_ssize_t n) {
         const at::Tensor& grad = tensor(o[0], "grad");
         a.grad_pitch = pitch_of(grad, "grad", device);
         same_matrix(grad, "grad", total, "total");
+        at::Tensor other;
         if (o[4] != Py_None) {
-            const at::Tensor& other = tensor(o[4], "grad_total");
+            other = tensor(o[4], "grad_total");
             a.grad_total_pitch = pitch_of(other, "grad_total", device);
             same_matrix(other, "grad_total", total, "total");
             a.grad_total = other.data_ptr();
         }
         a.gain = vector_of(o[2], "gain", a.width, device);
         a.rstd = vector_of(o[3], "rstd", a.rows, device);
+        const History history("rms_norm_backward", {{&grad, "grad"}, {&total, "total"}, {&THPVariable_Unpack(o[2]), "gain"},
+                                                    {&THPVariable_Unpack(o[3]), "rstd"}, {&other, "grad_total"}});
         at::Tensor grad_rows = empty({a.rows, a.width}, type, device), grad_gain = empty({a.width}, at::kFloat, device);
         if (a.width > 0) {
             a.workspace_bytes = mdx_hip_rms_norm_backward_workspace(a.rows, a.width);
@@ -312,6 +357,7 @@ PyObject* rms_norm_backward(PyObject*, PyObject* const* o, Py_ssize_t n) {
             void* stream = stream_of(device);
             run("rms_norm_backward", [&] { return mdx_hip_rms_norm_backward(device.index(), &a, stream); });
         }
+        history.goes_to({grad_rows, grad_gain});
         return tuple_of({grad_rows, grad_gain});
     });
 }
@@ -332,6 +378,7 @@ PyObject* quantize_fp8(PyObject*, PyObject* const* o, Py_ssize_t n) {
         a.tile = int32_t(whole(o[1]));
         a.transpose = PyObject_IsTrue(o[2]);
         if (a.transpose < 0) throw Raised{};
+        const History history("quantize_fp8", {{&matrix, "matrix"}});
         const int64_t down = a.transpose ? a.width : a.rows, across = a.transpose ? a.rows : a.width;
         at::Tensor codes = empty_codes(down, across, device);
         at::Tensor scales = empty_scales(ceil_div(down, a.tile), across, device);
@@ -344,6 +391,7 @@ PyObject* quantize_fp8(PyObject*, PyObject* const* o, Py_ssize_t n) {
             void* stream = stream_of(device);
             run("quantize_fp8", [&] { return mdx_hip_quantize_fp8(device.index(), &a, stream); });
         }
+        history.goes_to({codes, scales});
         return tuple_of({codes, scales});
     });
 }
@@ -398,6 +446,7 @@ PyObject* matmul_fp8(PyObject*, PyObject* const* o, Py_ssize_t n) {
             throw Refused{"b_scales must have shape " + shape_of({g.n, blocks}) + " or " + shape_of({tall, blocks})
                               + ", not " + shape_of(b.scales.sizes()),
                           "b_scales"};
+        const History history("matmul_fp8", {{&a.codes, "a"}, {&a.scales, "a_scales"}, {&b.codes, "b"}, {&b.scales, "b_scales"}});
         at::Tensor out;
         if (o[5] == Py_None) {
             const at::ScalarType type = type_of(o[4], "dtype must be a torch dtype");
@@ -410,6 +459,7 @@ PyObject* matmul_fp8(PyObject*, PyObject* const* o, Py_ssize_t n) {
             g.out_pitch = pitch_of(out, "out", device);
             if (out.size(0) != g.m || out.size(1) != g.n || kind_of(out.scalar_type()) < 0)
                 throw Refused{"out must be a float32, bfloat16 or float16 matrix of shape " + shape_of({g.m, g.n}), "out"};
+            history.refuse_out(out);
         }
         if (g.m > 0 && g.n > 0) {
             g.a = static_cast<const uint8_t*>(a.codes.data_ptr());
@@ -434,23 +484,23 @@ PyObject* matmul_fp8(PyObject*, PyObject* const* o, Py_ssize_t n) {
             run("matmul_fp8", [&] { return mdx_hip_matmul_fp8(device.index(), &g, stream); });
             if (o[5] != Py_None) written_to(out);
         }
+        history.goes_to({out});
         return THPVariable_Wrap(out);
     });
 }
 
-// A list or tuple of tensors, borrowed.
+// A list or tuple of tensors, held: the caller's list may change while a call lets go of Python.
 struct Tensors {
-    PyObject* fast = nullptr;
+    PyObject* held = nullptr;
     const char* name;
-    Tensors(PyObject* o, const char* n) : name(n) {
-        fast = PySequence_Fast(o, "a sequence of tensors is wanted");
-        if (fast == nullptr) throw Raised{};
+    Tensors(PyObject* o, const char* n) : held(PySequence_Tuple(o)), name(n) {
+        if (held == nullptr) throw Raised{};
     }
-    ~Tensors() { Py_XDECREF(fast); }
+    ~Tensors() { Py_XDECREF(held); }
     Tensors(const Tensors&) = delete;
     Tensors& operator=(const Tensors&) = delete;
-    Py_ssize_t size() const { return PySequence_Fast_GET_SIZE(fast); }
-    const at::Tensor& at(Py_ssize_t i) const { return tensor(PySequence_Fast_GET_ITEM(fast, i), name); }
+    Py_ssize_t size() const { return PyTuple_GET_SIZE(held); }
+    const at::Tensor& at(Py_ssize_t i) const { return tensor(PyTuple_GET_ITEM(held, i), name); }
 };
 
 // adamw_step(params, grads, first, second, first_scales, second_scales, step, lr, beta1, beta2, eps, decay, seed)
@@ -498,8 +548,6 @@ PyObject* adamw_step(PyObject*, PyObject* const* o, Py_ssize_t n) {
         std::vector<mdx_adamw_tensor> table(static_cast<size_t>(count));
         std::vector<void*> written;
         written.reserve(static_cast<size_t>(count) * 5);
-        std::vector<at::Tensor> moved; // held: the lists are the caller's, and may change while the call lets go of Python
-        moved.reserve(static_cast<size_t>(count) * 5);
         for (Py_ssize_t k = 0; k < count; ++k) {
             void* at_[6] = {};
             const at::Tensor& param = given[0]->at(k);
@@ -518,7 +566,6 @@ PyObject* adamw_step(PyObject*, PyObject* const* o, Py_ssize_t n) {
                     throw Refused{std::string(names[i]) + " must have the shapes of params", names[i]};
                 }
                 at_[i] = t.data_ptr();
-                if (i != 1) moved.push_back(t);
                 if (i != 1 && size > 0) written.push_back(at_[i]);
             }
             table[size_t(k)] = {size, static_cast<float*>(at_[0]), at_[1], at_[2], at_[3],
@@ -531,7 +578,8 @@ PyObject* adamw_step(PyObject*, PyObject* const* o, Py_ssize_t n) {
         a.count = count;
         void* stream = stream_of(device);
         run("adamw_step", [&] { return mdx_hip_adamw_step(device.index(), &a, stream); });
-        for (const at::Tensor& t : moved) written_to(t);
+        for (int i = 0; i < lists; ++i)
+            for (Py_ssize_t k = 0; i != 1 && k < count; ++k) written_to(given[i]->at(k));
         return none();
     });
 }

@@ -17,8 +17,14 @@ contiguous elements inside a row; rows may be pitched.  Every call queues its
 kernels on torch's current stream of that device and returns without waiting,
 keeps nothing for the next call, and can be captured into a graph; a tensor
 made on another stream is waited for, and its memory kept, as for any torch
-operation (``wait_stream``, ``record_stream``).  The functions do not record
-gradients themselves.
+operation (``wait_stream``, ``record_stream``).
+
+The functions record no gradients.  A ``torch.autograd.Function`` ties them
+together (``examples/energy_network.py`` holds one).  Outside of one, with
+grad mode on, results of inputs that require gradients raise when a backward
+pass reaches them; an ``out`` is then refused, and so are forward gradients.
+Tensors that a call writes get a new version, so that a graph that has saved
+one raises.
 
 A float8 matrix is a pair: codes of type ``torch.float8_e4m3fn`` and scales of
 type ``torch.float8_e8m0fnu``, powers of two.  An element stands for its code

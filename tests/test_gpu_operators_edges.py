@@ -275,3 +275,56 @@ def test_tensors_of_inference_mode_are_written_too():
         p = torch.zeros(100, device="cuda")
         mdx.adamw_step([p], [torch.ones(100, device="cuda")], *mdx.adamw_state([p], bits=8), step=1, lr=0.5)
     assert torch.equal(out, mdx.matmul_fp8(codes, scales, codes, scales, dtype=torch.float32)) and torch.all(p < -0.49)
+
+
+def recorded_calls():
+    """Each call with one input that requires gradients, and the input."""
+
+    x, gain = randn(50, 20, 256), randn(51, 256)
+    rstd = torch.ones(20, device="cuda")
+    codes, scales = mdx.quantize_fp8(x)
+
+    def leaf(t):
+        return t.clone().requires_grad_()
+
+    for v in (leaf(x),):
+        yield "norm of rows", v, lambda v=v: mdx.rms_norm(v, gain).values
+        yield "norm's total", v, lambda v=v: mdx.rms_norm(x, gain, residual=v).total
+        yield "norm's rstd", v, lambda v=v: mdx.rms_norm(v, gain).rstd
+        yield "norm to codes", v, lambda v=v: mdx.rms_norm(v, gain, dtype=CODES).values
+        yield "codes", v, lambda v=v: mdx.quantize_fp8(v)[0]
+        yield "product of codes", v, lambda v=v: mdx.matmul_fp8(*mdx.quantize_fp8(v), codes, scales)
+        yield "gradients", v, lambda v=v: mdx.rms_norm_backward(v, x, gain, rstd)[0]
+        yield "gradients' total", v, lambda v=v: mdx.rms_norm_backward(x, x, gain, rstd, grad_total=v)[1]
+    w = leaf(gain)
+    yield "norm's gain", w, lambda: mdx.rms_norm(x, w, dtype=CODES).values
+
+
+def test_gradients_are_not_lost_in_silence():
+    """A sum of a call's result and another way: the backward pass raises, it does not leave the call's part out."""
+
+    for name, v, run in recorded_calls():
+        out = run()
+        assert out.requires_grad, name
+        with pytest.raises(RuntimeError, match="records no gradients"):
+            (out.float().sum() + v.sum()).backward()
+        with torch.no_grad():
+            assert not run().requires_grad, name
+
+
+def test_out_and_forward_gradients_are_refused_where_gradients_are_recorded():
+    x, gain = randn(52, 20, 256), randn(53, 256)
+    v = x.clone().requires_grad_()
+    codes, scales = mdx.quantize_fp8(x)
+    out = torch.zeros(20, 20, device="cuda")
+    with pytest.raises(mdx.DescriptorInputError, match="out records no gradients"):
+        mdx.matmul_fp8(*mdx.quantize_fp8(v), codes, scales, out=out)
+    with pytest.raises(mdx.DescriptorInputError, match="out requires gradients"):
+        mdx.matmul_fp8(codes, scales, codes, scales, out=out.clone().requires_grad_())
+    with torch.no_grad():
+        mdx.matmul_fp8(*mdx.quantize_fp8(v), codes, scales, out=out)
+    assert torch.equal(out, mdx.matmul_fp8(codes, scales, codes, scales, dtype=torch.float32))
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises(mdx.DescriptorInputError, match="forward gradient"):
+            mdx.rms_norm(dual, gain)
