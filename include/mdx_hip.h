@@ -342,7 +342,7 @@ void mdx_hip_host_free(void* ptr);
  * the structs themselves are host memory and are read before the call
  * returns.  Each call only queues kernels on `stream` (a hipStream_t; NULL is
  * the default stream) and allocates nothing, so it can be captured into a
- * graph and calls on different streams do not wait for each other.  Calls
+ * graph (whose replays repeat its numbers: see mdx_adamw_args), and calls on different streams do not wait for each other.  Calls
  * keep nothing: a workspace is the caller's and is free again when the
  * stream has passed the call.  A workspace of sizes that the call refuses has
  * zero bytes.  Errors: mdx_hip_last_error(NULL), per thread.
@@ -478,7 +478,14 @@ int mdx_hip_matmul_fp8(int device, const mdx_matmul_args* args, void* stream);
  *   mix(lo(i) ^ mix(seed + 0x9E3779B9 (tensor + 1) + 0x85EBCA6B hi(i))),
  * i the element's place in its tensor, tensor the tensor's place in the list
  * and mix the 32-bit x ^= x >> 16, x *= 0x6A09E667, x ^= x >> 15,
- * x *= 0xBB67AE85, x ^= x >> 16: the result depends on the inputs alone. */
+ * x *= 0xBB67AE85, x ^= x >> 16: the result depends on the inputs alone.
+ *
+ * A graph that has captured the call repeats its numbers on every replay: the
+ * same step, the same bias corrections and the same random bits, by which v
+ * would stand still after all.  step_at and seed_at (each may be NULL) are
+ * device addresses of numbers that are read in place of step and seed when the
+ * kernels run (of the seed the low 32 bits), so that a replay goes on with what the
+ * graph or its caller has written there.  A step below 1 there changes nothing. */
 typedef struct mdx_adamw_tensor {
     int64_t n;
     float* params;
@@ -496,6 +503,8 @@ typedef struct mdx_adamw_args {
     uint32_t seed;
     int32_t grad_dtype;
     int32_t bits;
+    const int64_t* step_at;
+    const int64_t* seed_at;
 } mdx_adamw_args;
 int mdx_hip_adamw_step(int device, const mdx_adamw_args* args, void* stream);
 

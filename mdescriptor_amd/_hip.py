@@ -302,6 +302,8 @@ class AdamwArgs(ctypes.Structure):
         ("seed", ctypes.c_uint32),
         ("grad_dtype", ctypes.c_int32),
         ("bits", ctypes.c_int32),
+        ("step_at", ctypes.c_void_p),
+        ("seed_at", ctypes.c_void_p),
     ]
 
 

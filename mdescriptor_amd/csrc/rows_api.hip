@@ -181,7 +181,9 @@ int mdx_hip_adamw_step(int device, const mdx_adamw_args* args, void* stream) {
         require(g.bits == 8 || g.bits == 32, "states have 8 or 32 bits");
         require(g.count >= 0 && g.count < kMostRows && (g.count == 0 || g.tensors != nullptr),
                 "the tensors must not be null");
-        require(g.step >= 1, "step must be at least 1");
+        require(g.step_at != nullptr || g.step >= 1, "step must be at least 1");
+        require(reinterpret_cast<uintptr_t>(g.step_at) % 8 == 0 && reinterpret_cast<uintptr_t>(g.seed_at) % 8 == 0,
+                "step_at and seed_at must be aligned to their numbers");
         require(std::isfinite(g.lr) && g.lr >= 0.0, "lr must be finite and not negative");
         require(g.beta1 >= 0.0 && g.beta1 < 1.0 && g.beta2 >= 0.0 && g.beta2 < 1.0, "betas must lie in [0, 1)");
         require(std::isfinite(g.eps) && float(g.eps) > 0.0f, "eps must be positive and finite");

@@ -114,6 +114,18 @@ float* vector_of(PyObject* o, const char* name, int64_t size, at::Device device)
     return static_cast<float*>(t.data_ptr());
 }
 
+// Whether a number is one that the device reads: other tensors of one element are numbers as Python takes them.
+bool moves(PyObject* o) {
+    return THPVariable_Check(o) && THPVariable_Unpack(o).is_cuda() && THPVariable_Unpack(o).scalar_type() == at::kLong;
+}
+
+const int64_t* number_at(PyObject* o, const char* name, at::Device device) {
+    const at::Tensor& t = THPVariable_Unpack(o);
+    if (t.device() != device || t.numel() != 1)
+        throw Refused{std::string(name) + " must be a whole number or an int64 tensor of one element on " + device.str(), name};
+    return static_cast<const int64_t*>(t.data_ptr());
+}
+
 at::Tensor empty(at::IntArrayRef shape, at::ScalarType type, at::Device device) {
     return at::detail::empty_cuda(shape, type, device, std::nullopt); // past the dispatcher: 0.3 us less each
 }
@@ -521,13 +533,14 @@ PyObject* adamw_step(PyObject*, PyObject* const* o, Py_ssize_t n) {
                                   + " params",
                               names[i]};
         mdx_adamw_args a{};
-        a.step = whole(o[6]);
+        const bool moving_step = moves(o[6]), moving_seed = moves(o[12]);
+        a.step = moving_step ? 1 : whole(o[6]);
         a.lr = number(o[7]);
         a.beta1 = number(o[8]);
         a.beta2 = number(o[9]);
         a.eps = number(o[10]);
         a.weight_decay = number(o[11]);
-        a.seed = uint32_t(PyLong_AsUnsignedLongLongMask(o[12]));
+        if (!moving_seed) a.seed = uint32_t(PyLong_AsUnsignedLongLongMask(o[12]));
         if (PyErr_Occurred()) throw Raised{};
         a.bits = eight ? 8 : 32;
         if (a.step < 1) throw Refused{"step must be a whole number from 1 on", "step"};
@@ -540,6 +553,8 @@ PyObject* adamw_step(PyObject*, PyObject* const* o, Py_ssize_t n) {
         const at::Tensor& lead = given[0]->at(0);
         if (!lead.is_cuda()) throw Refused{"params must live on a HIP device", "params"};
         const at::Device device = lead.device();
+        if (moving_step) a.step_at = number_at(o[6], "step", device);
+        if (moving_seed) a.seed_at = number_at(o[12], "seed", device);
         const at::ScalarType grad_type = given[1]->at(0).scalar_type();
         if (kind_of(grad_type) < 0) throw Refused{"grads must be float32, bfloat16 or float16 tensors", "grads"};
         a.grad_dtype = kind_of(grad_type);

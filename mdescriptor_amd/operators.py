@@ -15,9 +15,10 @@ whose results leave for host memory.
 Arrays are torch tensors on one HIP device.  Matrices are two-dimensional with
 contiguous elements inside a row; rows may be pitched.  Every call queues its
 kernels on torch's current stream of that device and returns without waiting,
-keeps nothing for the next call, and can be captured into a graph; a tensor
-made on another stream is waited for, and its memory kept, as for any torch
-operation (``wait_stream``, ``record_stream``).
+keeps nothing for the next call, and can be captured into a graph.  Replays
+repeat the call's numbers; :func:`adamw_step` takes those that a step moves as
+tensors too.  A tensor made on another stream is waited for, and its memory
+kept, as for any torch operation (``wait_stream``, ``record_stream``).
 
 The functions record no gradients.  A ``torch.autograd.Function`` ties them
 together (``examples/energy_network.py`` holds one).  Outside of one, with
@@ -193,9 +194,9 @@ def adamw_state(params: Sequence[torch.Tensor], *, bits: int = 32) -> AdamwState
 
 def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], first: Sequence[torch.Tensor],
                second: Sequence[torch.Tensor], first_scales: Sequence[torch.Tensor] | None = None,
-               second_scales: Sequence[torch.Tensor] | None = None, *, step: int, lr: float = 1e-3,
+               second_scales: Sequence[torch.Tensor] | None = None, *, step: int | torch.Tensor, lr: float = 1e-3,
                betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01,
-               seed: int = 0) -> None:
+               seed: int | torch.Tensor = 0) -> None:
     """One AdamW step over many contiguous tensors, in place::
 
         m = beta1 * m + (1 - beta1) * g;  v = beta2 * v + (1 - beta2) * g**2
@@ -208,9 +209,19 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], fi
     without bias, from ``seed`` (give each step its own), the tensor's place
     in the list and the element's place in it: rounded to nearest they would
     never move, since a step changes v by less than half of a code.  ``step``
-    counts from 1.  An infinite or NaN gradient spoils its element's moments,
-    in 8 bits its block's.  The root and the quotient are good to one unit in
-    the last place; a v below float32's normal numbers has the root zero."""
+    counts from 1.
+
+    ``step`` and ``seed`` may be int64 tensors of one element on the device,
+    read when the kernels run.  A captured step needs them: a replay repeats
+    numbers, and with them the first step's bias corrections and random
+    bits, by which v would stand still after all.  Move them in the graph
+    (``step.add_(1)``), or write them before each replay; one tensor can be
+    both.  A step below 1 there changes nothing.  ``lr`` and the other numbers
+    stay those of the captured call.
+
+    An infinite or NaN gradient spoils its element's moments, in 8 bits its
+    block's.  The root and the quotient are good to one unit in the last
+    place; a v below float32's normal numbers has the root zero."""
 
     _calls.adamw_step(params, grads, first, second, first_scales, second_scales, step, lr, betas[0], betas[1], eps,
                       weight_decay, seed)

@@ -328,3 +328,103 @@ def test_out_and_forward_gradients_are_refused_where_gradients_are_recorded():
         dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
         with pytest.raises(mdx.DescriptorInputError, match="forward gradient"):
             mdx.rms_norm(dual, gain)
+
+
+# ------------------------------------------------ steps in a replayed graph
+
+def number(value: int) -> torch.Tensor:
+    return torch.tensor([value], dtype=torch.int64, device="cuda")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("bits", [8, 32])
+def test_replays_of_a_captured_step_are_successive_steps(dtype, bits):
+    """One captured step that moves its own step and seed on, replayed, against eager steps with numbers.  The moments do not
+    depend on the bias corrections: the same bits.  The corrections are rounded from float64, so the update is the
+    same to a unit in the last place, 2 u, of either factor, and its difference to the roundings that follow."""
+
+    sizes = (1, 130, 5000)
+    start = [randn(60 + i, n) for i, n in enumerate(sizes)]
+    grads = [0.01 * randn(70 + i, n) for i, n in enumerate(sizes)]
+    grads = [g.to(dtype) for g in grads]
+    lr = 1e-2
+    eager, replayed = ([p.clone() for p in start] for _ in range(2))
+    states = [mdx.adamw_state(eager, bits=bits) for _ in range(2)]
+    step = number(0)
+
+    def move():
+        step.add_(1)
+        mdx.adamw_step(replayed, grads, *states[1], step=step, seed=step, lr=lr)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):  # once before the capture: the first step
+        move()
+    torch.cuda.current_stream().wait_stream(side)
+    mdx.adamw_step(eager, grads, *states[0], step=1, seed=1, lr=lr)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        move()
+    for turn in range(2, 8):
+        graph.replay()
+        mdx.adamw_step(eager, grads, *states[0], step=turn, seed=turn, lr=lr)
+        torch.cuda.synchronize()
+        assert int(step) == turn
+        for parts in zip(*states):
+            for want, got in zip(*parts) if parts[0] is not None else ():
+                assert torch.equal(raw(got), raw(want))
+        for want, got in zip(eager, replayed):
+            # an update is at most lr sqrt(1 / (1 - beta2)) = 32 lr
+            assert torch.all((got - want).abs() <= turn * (8 * U * 32 * lr + 2 * U * want.abs()))
+
+
+@pytest.mark.parametrize("step", [1, 2, 1000, 10 ** 6, 2 ** 40])
+@pytest.mark.parametrize("betas", [(0.9, 0.999), (0.0, 0.0), (0.5, 0.9999999)])
+def test_a_step_in_device_memory_is_the_step(step, betas):
+    grad, lr = randn(80, 700), 1e-2
+    results = []
+    for at in (step, number(step), torch.tensor(step), torch.tensor([step], dtype=torch.int64)):  # the latter are numbers
+        p = randn(81, 700)
+        state = mdx.adamw_state([p])
+        mdx.adamw_step([p], [grad], *state, step=at, lr=lr, betas=betas)
+        results.append((p, state.first[0], state.second[0]))
+    want = results[0]
+    for got in results[1:]:
+        assert torch.equal(got[1], want[1]) and torch.equal(got[2], want[2])
+        # the update m / (1 - beta1^step) / sqrt(v / (1 - beta2^step)) is at most 1 / sqrt(1 - beta2) here
+        moved = lr / math.sqrt(1.0 - betas[1])
+        assert torch.all((got[0] - want[0]).abs() <= 8 * U * moved + 2 * U * want[0].abs())
+    for got in results[2:]:
+        assert torch.equal(got[0], want[0])
+
+
+def test_a_seed_in_device_memory_is_the_seed():
+    grad = randn(82, 5000)
+    for seed in (0, 7, -3, 2 ** 32 - 1, 2 ** 33 + 5):
+        codes = []
+        for at in (seed, number(seed)):
+            p = randn(83, 5000)
+            state = mdx.adamw_state([p], bits=8)
+            mdx.adamw_step([p], [grad], *state, step=2, seed=at)
+            codes.append((p, raw(state.first[0]), raw(state.second[0])))
+        assert all(torch.equal(a, b) for a, b in zip(*codes))
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_step_below_one_in_device_memory_changes_nothing(bits):
+    p, grad = randn(84, 300), randn(85, 300)
+    state = mdx.adamw_state([p], bits=bits)
+    mdx.adamw_step([p], [grad], *state, step=1)
+    before = [t.clone() for t in (p, *(part[0] for part in state if part is not None))]
+    for at in (0, -1):
+        mdx.adamw_step([p], [grad], *state, step=number(at))
+    after = (p, *(part[0] for part in state if part is not None))
+    assert all(torch.equal(raw(a), raw(b)) for a, b in zip(before, after))
+
+
+def test_numbers_in_device_memory_are_refused_where_they_are_not_one():
+    p = randn(86, 30)
+    state = mdx.adamw_state([p])
+    for name in ("step", "seed"):
+        with pytest.raises(mdx.DescriptorInputError, match=f"{name} must be a whole number or an int64 tensor"):
+            mdx.adamw_step([p], [p.clone()], *state, **{"step": 1, name: torch.ones(2, dtype=torch.int64, device="cuda")})

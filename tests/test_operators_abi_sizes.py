@@ -69,3 +69,14 @@ def test_adamw_refuses_tensors_of_more_than_one_launch(hip):
                              weight_decay=0.0, step=1, seed=0, grad_dtype=1, bits=8)
         assert lib.mdx_hip_adamw_step(0, ctypes.byref(args), None) == hip.MDX_INVALID_ARGUMENT
         assert "size" in lib.mdx_hip_last_error(None).decode()
+
+
+def test_adamw_takes_a_step_from_device_memory_in_place_of_the_number(hip):
+    lib = hip.load_library()
+    values = dict(tensors=None, count=0, lr=1e-3, beta1=0.9, beta2=0.99, eps=1e-8, weight_decay=0.0, step=0, seed=0,
+                  grad_dtype=0, bits=32)
+    call = lambda **c: lib.mdx_hip_adamw_step(0, ctypes.byref(hip.AdamwArgs(**{**values, **c})), None)  # noqa: E731
+    assert call() == hip.MDX_INVALID_ARGUMENT and "step must" in lib.mdx_hip_last_error(None).decode()
+    for name in ("step_at", "seed_at"):
+        assert call(**{"step": 1, name: P + 4}) == hip.MDX_INVALID_ARGUMENT
+        assert "aligned" in lib.mdx_hip_last_error(None).decode()
