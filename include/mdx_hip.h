@@ -468,6 +468,9 @@ int mdx_hip_matmul_fp8(int device, const mdx_matmul_args* args, void* stream);
  *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,
  *   p = p (1 - lr weight_decay) - lr / (1 - beta1^step) *
  *       m / (sqrt(v / (1 - beta2^step)) + eps).
+ * Tensors have at most 2^35 - 2^11 elements; those that are written overlap
+ * neither each other nor gradients (grads may be its own params or float32
+ * moments).
  * params and (bits 32) first = m, second = v are f32[n]; grads have
  * grad_dtype.  With bits 8 first and second hold float8 codes of m and of
  * sqrt(v), with one scale per 128 elements in first_scales and second_scales:

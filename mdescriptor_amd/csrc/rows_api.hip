@@ -4,7 +4,10 @@
 // and no call waits, so each may be captured into a graph.
 #include "rows_device.h"
 
+#include <algorithm>
 #include <cmath>
+#include <utility>
+#include <vector>
 
 #include "rows_internal.h"
 
@@ -60,6 +63,41 @@ void check_codes(const uint8_t* codes, int64_t pitch, int64_t width, const uint8
     require(pitch % 128 == 0 && pitch >= width, "the pitch of written codes must be a multiple of 128");
     require(reinterpret_cast<uintptr_t>(codes) % 16 == 0, "written codes must be 16-byte aligned");
     require(scales_pitch >= (width + 127) / 128, "the pitch of the scales is below their number");
+}
+
+// What a step writes may be read or written by its own lanes alone: workgroups run in any order.
+void check_apart(const mdx_adamw_args& g) {
+    typedef std::pair<uintptr_t, uintptr_t> Range; // bytes from and up to
+    std::vector<Range> written;
+    written.reserve(size_t(g.count) * 5);
+    auto range = [](const void* p, int64_t bytes) {
+        const uintptr_t from = reinterpret_cast<uintptr_t>(p);
+        return Range(from, from + uintptr_t(bytes));
+    };
+    const int64_t state = g.bits == 8 ? 1 : 4;
+    for (int64_t i = 0; i < g.count; ++i) {
+        const mdx_adamw_tensor& x = g.tensors[i];
+        if (x.n == 0) continue;
+        written.push_back(range(x.params, x.n * 4));
+        written.push_back(range(x.first, x.n * state));
+        written.push_back(range(x.second, x.n * state));
+        if (g.bits == 32) continue;
+        written.push_back(range(x.first_scales, (x.n + 127) / 128));
+        written.push_back(range(x.second_scales, (x.n + 127) / 128));
+    }
+    std::sort(written.begin(), written.end());
+    for (size_t i = 1; i < written.size(); ++i)
+        require(written[i].first >= written[i - 1].second, "a tensor that the step writes is given twice, or overlaps another");
+    const int64_t size = element_size(g.grad_dtype);
+    for (int64_t i = 0; i < g.count; ++i) {
+        const mdx_adamw_tensor& x = g.tensors[i];
+        // in the very place of its own tensor each lane reads before it writes
+        if (x.n == 0 || (size == 4 && (x.grads == x.params || (state == 4 && (x.grads == x.first || x.grads == x.second)))))
+            continue;
+        const Range r = range(x.grads, x.n * size);
+        const auto after = std::lower_bound(written.begin(), written.end(), Range(r.second, 0)); // the first from its end on
+        require(after == written.begin() || std::prev(after)->second <= r.first, "a gradient overlaps what the step writes");
+    }
 }
 
 } // namespace
@@ -199,6 +237,7 @@ int mdx_hip_adamw_step(int device, const mdx_adamw_args* args, void* stream) {
             require(g.bits == 32 || (x.first_scales != nullptr && x.second_scales != nullptr),
                     "states in 8 bits need scales");
         }
+        check_apart(g);
         OnDevice on(device);
         mdx::adamw_step(g, static_cast<hipStream_t>(stream));
     });

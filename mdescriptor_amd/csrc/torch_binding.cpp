@@ -561,8 +561,6 @@ PyObject* adamw_step(PyObject*, PyObject* const* o, Py_ssize_t n) {
         const at::ScalarType state = eight ? kCodes : at::kFloat;
         const at::ScalarType types[6] = {at::kFloat, grad_type, state, state, kScales, kScales};
         std::vector<mdx_adamw_tensor> table(static_cast<size_t>(count));
-        std::vector<void*> written;
-        written.reserve(static_cast<size_t>(count) * 5);
         for (Py_ssize_t k = 0; k < count; ++k) {
             void* at_[6] = {};
             const at::Tensor& param = given[0]->at(k);
@@ -581,14 +579,10 @@ PyObject* adamw_step(PyObject*, PyObject* const* o, Py_ssize_t n) {
                     throw Refused{std::string(names[i]) + " must have the shapes of params", names[i]};
                 }
                 at_[i] = t.data_ptr();
-                if (i != 1 && size > 0) written.push_back(at_[i]);
             }
             table[size_t(k)] = {size, static_cast<float*>(at_[0]), at_[1], at_[2], at_[3],
                                 static_cast<uint8_t*>(at_[4]), static_cast<uint8_t*>(at_[5])};
         }
-        std::sort(written.begin(), written.end());
-        if (std::adjacent_find(written.begin(), written.end()) != written.end())
-            throw Refused{"a tensor that the step writes is given twice", "params"};
         a.tensors = table.data();
         a.count = count;
         void* stream = stream_of(device);

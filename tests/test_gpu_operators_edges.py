@@ -428,3 +428,19 @@ def test_numbers_in_device_memory_are_refused_where_they_are_not_one():
     for name in ("step", "seed"):
         with pytest.raises(mdx.DescriptorInputError, match=f"{name} must be a whole number or an int64 tensor"):
             mdx.adamw_step([p], [p.clone()], *state, **{"step": 1, name: torch.ones(2, dtype=torch.int64, device="cuda")})
+
+
+def test_a_step_over_tensors_that_overlap_is_refused():
+    flat, grad = randn(87, 1000), randn(88, 300)
+    for first in (flat[200:500], flat[299:599]):
+        with pytest.raises(mdx.DescriptorInputError, match="overlaps"):
+            mdx.adamw_step([flat[:300]], [grad], [first], [torch.zeros_like(grad)], step=1)
+    with pytest.raises(mdx.DescriptorInputError, match="gradient overlaps"):
+        mdx.adamw_step([flat[:300]], [flat[1:301]], [grad], [torch.zeros_like(grad)], step=1)
+    # side by side, and with the gradient in its parameter's own place
+    p = [flat[:300], flat[300:600]]
+    g = [flat[:300], grad]
+    want = [x.clone() for x in p]
+    mdx.adamw_step(want, [x.clone() for x in g], *mdx.adamw_state(want), step=1)
+    mdx.adamw_step(p, g, *mdx.adamw_state(p), step=1)
+    assert all(torch.equal(a, b) for a, b in zip(p, want))

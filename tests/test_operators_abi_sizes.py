@@ -80,3 +80,39 @@ def test_adamw_takes_a_step_from_device_memory_in_place_of_the_number(hip):
     for name in ("step_at", "seed_at"):
         assert call(**{"step": 1, name: P + 4}) == hip.MDX_INVALID_ARGUMENT
         assert "aligned" in lib.mdx_hip_last_error(None).decode()
+
+
+M = 1 << 20  # addresses far apart that nothing here reads
+
+
+@pytest.mark.parametrize("bits, places, apart", [
+    # (params, grads, first, second, first_scales, second_scales) of tensors of 200 elements
+    (32, [(M, 2 * M, 3 * M, 4 * M)], True),
+    (32, [(M, M, 3 * M, 4 * M)], True),                      # the gradient in its parameter's place
+    (32, [(M, 3 * M, 3 * M, 4 * M)], True),                  # or in a float32 moment's
+    (32, [(M, 2 * M, M, 4 * M)], False),
+    (32, [(M, 2 * M, M + 796, 4 * M)], False),               # the last element of one is the first of the other
+    (32, [(M, 2 * M, M + 800, 4 * M)], True),
+    (32, [(M, M + 4, 3 * M, 4 * M)], False),                 # a gradient one element off
+    (32, [(M, 3 * M - 796, 3 * M, 4 * M)], False),
+    (32, [(M, 3 * M - 800, 3 * M, 4 * M)], True),
+    (32, [(M, 2 * M, 3 * M, 4 * M), (M + 400, 2 * M, 5 * M, 6 * M)], False),
+    (32, [(M, 2 * M, 3 * M, 4 * M), (7 * M, 2 * M + 4, 5 * M, 6 * M)], True),  # gradients may share
+    (32, [(M, 2 * M, 3 * M, 4 * M), (7 * M, M, 5 * M, 6 * M)], False),         # another tensor's parameter
+    (8, [(M, 2 * M, 3 * M, 4 * M, 5 * M, 6 * M)], True),
+    (8, [(M, 2 * M, 3 * M, 3 * M + 199, 5 * M, 6 * M)], False),
+    (8, [(M, 2 * M, 3 * M, 3 * M + 200, 5 * M, 6 * M)], True),
+    (8, [(M, 2 * M, 3 * M, 4 * M, 5 * M, 5 * M + 1)], False),
+    (8, [(M, 2 * M, 3 * M, 4 * M, 5 * M, 5 * M + 2)], True),
+    (8, [(M, 3 * M, 3 * M, 4 * M, 5 * M, 6 * M)], False),    # codes are not where a float32 gradient is read
+])
+def test_adamw_refuses_tensors_that_overlap(hip, bits, places, apart):
+    """On a device that is not there, so that what is not refused for this goes no further."""
+
+    lib = hip.load_library()
+    table = (hip.AdamwTensor * len(places))(*(hip.AdamwTensor(200, *place) for place in places))
+    args = hip.AdamwArgs(tensors=ctypes.addressof(table), count=len(places), lr=1e-3, beta1=0.9, beta2=0.99, eps=1e-8,
+                         weight_decay=0.0, step=1, seed=0, grad_dtype=0, bits=bits)
+    status = lib.mdx_hip_adamw_step(12345, ctypes.byref(args), None)
+    message = lib.mdx_hip_last_error(None).decode()
+    assert status != hip.MDX_OK and ("overlaps" not in message) == apart, message
