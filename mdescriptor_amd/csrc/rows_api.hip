@@ -224,7 +224,8 @@ int mdx_hip_adamw_step(int device, const mdx_adamw_args* args, void* stream) {
                 "step_at and seed_at must be aligned to their numbers");
         require(std::isfinite(g.lr) && g.lr >= 0.0, "lr must be finite and not negative");
         require(g.beta1 >= 0.0 && g.beta1 < 1.0 && g.beta2 >= 0.0 && g.beta2 < 1.0, "betas must lie in [0, 1)");
-        require(std::isfinite(g.eps) && float(g.eps) > 0.0f, "eps must be positive and finite");
+        // the kernel multiplies by the device's reciprocal, which is infinite below the normal numbers
+        require(std::isfinite(g.eps) && float(g.eps) >= 0x1p-126f, "eps must be finite and at least 2^-126");
         require(std::isfinite(g.weight_decay) && g.weight_decay >= 0.0, "weight_decay must be finite and not negative");
         for (int64_t i = 0; i < g.count; ++i) {
             const mdx_adamw_tensor& x = g.tensors[i];

@@ -221,7 +221,8 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], fi
 
     An infinite or NaN gradient spoils its element's moments, in 8 bits its
     block's.  The root and the quotient are good to one unit in the last
-    place; a v below float32's normal numbers has the root zero."""
+    place; a v below float32's normal numbers has the root zero.  ``eps`` is
+    2**-126 at least."""
 
     _calls.adamw_step(params, grads, first, second, first_scales, second_scales, step, lr, betas[0], betas[1], eps,
                       weight_decay, seed)

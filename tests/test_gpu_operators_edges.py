@@ -444,3 +444,16 @@ def test_a_step_over_tensors_that_overlap_is_refused():
     mdx.adamw_step(want, [x.clone() for x in g], *mdx.adamw_state(want), step=1)
     mdx.adamw_step(p, g, *mdx.adamw_state(p), step=1)
     assert all(torch.equal(a, b) for a, b in zip(p, want))
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_step_of_zero_gradients_with_the_smallest_eps(bits):
+    """0 / (0 + eps) is zero: the parameters decay and nothing else."""
+
+    p, g = randn(89, 300), torch.zeros(300, device="cuda")
+    for eps in (2.0 ** -126, 1e-30, 1e-8):
+        q = p.clone()
+        mdx.adamw_step([q], [g], *mdx.adamw_state([q], bits=bits), step=1, eps=eps, lr=0.5, weight_decay=0.5)
+        assert torch.equal(q, 0.75 * p)
+    with pytest.raises(mdx.DescriptorInputError, match="eps"):
+        mdx.adamw_step([p], [g], *mdx.adamw_state([p], bits=bits), step=1, eps=1e-39)

@@ -116,3 +116,15 @@ def test_adamw_refuses_tensors_that_overlap(hip, bits, places, apart):
     status = lib.mdx_hip_adamw_step(12345, ctypes.byref(args), None)
     message = lib.mdx_hip_last_error(None).decode()
     assert status != hip.MDX_OK and ("overlaps" not in message) == apart, message
+
+
+@pytest.mark.parametrize("eps", [1e-45, 1e-39, 1.1754942e-38])
+def test_adamw_refuses_an_eps_whose_quotient_is_infinite(hip, eps):
+    """1 / eps is infinite below float32's normal numbers, and the zero moment of a zero gradient times it NaN."""
+
+    lib = hip.load_library()
+    table = (hip.AdamwTensor * 1)(hip.AdamwTensor(200, M, 2 * M, 3 * M, 4 * M))
+    args = hip.AdamwArgs(tensors=ctypes.addressof(table), count=1, lr=1e-3, beta1=0.9, beta2=0.99, eps=eps,
+                         weight_decay=0.0, step=1, seed=0, grad_dtype=0, bits=32)
+    assert lib.mdx_hip_adamw_step(12345, ctypes.byref(args), None) == hip.MDX_INVALID_ARGUMENT
+    assert "eps" in lib.mdx_hip_last_error(None).decode()
