@@ -163,10 +163,14 @@ def matmul_fp8(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scale
     quantised transposes of the output's gradient and of the input.  ``out``
     may be given, with pitched rows too; its type is then the result's.
 
-    Float32 results lose nothing but float32's own roundings.  For 16-bit
-    results the device's float8 products are taken, which add each eight
-    neighbouring products as multiples of 2**-13 of the largest of them before
-    they go on in float32 (1.6e-5 of a result of random signs, at any length)."""
+    Float32 results lose nothing but float32's own roundings, where the
+    elements (code times scale) lie in bfloat16's range: those of scales from
+    2**-124 to 2**119 do, and :func:`quantize_fp8` gives no others.  For 16-bit
+    results, at any scales, the device's float8 products are taken, which add
+    each eight neighbouring products as multiples of 2**-13 of the largest of
+    them before they go on in float32: at most 7 * 2**-13 of the sum of those
+    largest ones; 1.6e-5 of a result of random signs, at any length, and 7e-6
+    of one of equal signs as measured."""
 
     return _calls.matmul_fp8(a, a_scales, b, b_scales, dtype, out)
 

@@ -457,3 +457,80 @@ def test_a_step_of_zero_gradients_with_the_smallest_eps(bits):
         assert torch.equal(q, 0.75 * p)
     with pytest.raises(mdx.DescriptorInputError, match="eps"):
         mdx.adamw_step([p], [g], *mdx.adamw_state([p], bits=bits), step=1, eps=1e-39)
+
+
+# -------------------------------------------------- precision of products
+
+SHAPES = [(5, 24, 200), (70, 90, 300), (300, 300, 1000)]  # the kernel for few rows, and tiles
+
+
+def whole_codes(seed: int, rows: int, k: int) -> torch.Tensor:
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randint(-15, 16, (rows, k), generator=g, device="cuda").float()
+
+
+def one_scale(rows: int, k: int, byte: int) -> torch.Tensor:
+    return torch.full((rows, -(-k // 128)), byte, dtype=torch.uint8, device="cuda").view(SCALES)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+def test_product_at_every_scale(dtype, shape):
+    """Scales 2^e and 2^-e of whole numbers: exact.  16-bit results take every scale there is, float32 ones those whose
+    elements bfloat16 holds: 15 * 2^124 is below 2^128, 15 * 2^-124 a multiple of 2^-133."""
+
+    m, n, k = shape
+    a, b = whole_codes(90, m, k), whole_codes(91, n, k)
+    want = (a.double() @ b.double().T.contiguous()).to(dtype)
+    for byte in range(3, 252) if dtype == torch.float32 else range(255):
+        got = mdx.matmul_fp8(a.to(CODES), one_scale(m, k, byte), b.to(CODES), one_scale(n, k, 254 - byte), dtype=dtype)
+        assert torch.equal(got, want), byte
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+def test_float32_product_of_the_largest_and_smallest_elements(shape):
+    """Every code at the ends of the documented scales: 448 * 2^119 with multiples of 2^-9 * 2^-124.  Exact: products are
+    whole multiples of 7 * 2^-8, below 2^24 of them."""
+
+    m, n, k = shape
+    a, b = 448.0 * whole_codes(92, m, k).sign(), whole_codes(93, n, k) * 2.0 ** -9
+    want = a.double() @ b.double().T.contiguous() * 2.0 ** -5
+    for first, second in (((a, 246), (b, 3)), ((b, 3), (a, 246))):
+        (x, xs), (y, ys) = first, second
+        got = mdx.matmul_fp8(x.to(CODES), one_scale(len(x), k, xs), y.to(CODES), one_scale(len(y), k, ys), dtype=torch.float32)
+        assert torch.equal(got, (want if x is a else want.T).float())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+def test_product_of_blocks_of_zeros_at_any_scale(dtype, shape):
+    """Zero codes stand for zeros whatever their scale's byte, NaN apart."""
+
+    m, n, k = shape
+    a, b = whole_codes(94, m, k), whole_codes(95, n, k)
+    a[:, :128] = 0.0
+    want = (a.double() @ b.double().T.contiguous()).to(dtype)
+    for byte in (0, 1, 253, 254):
+        scales = one_scale(m, k, 127).clone()
+        scales.view(torch.uint8)[:, 0] = byte
+        got = mdx.matmul_fp8(a.to(CODES), scales, b.to(CODES), one_scale(n, k, 127), dtype=dtype)
+        assert torch.equal(got, want), byte
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(70, 90, 300), (130, 200, 8000)])
+def test_product_of_equal_signs(dtype, shape):
+    """Operands without a sign, as features often are: nothing cancels what the groups of eight lose, at most 7 * 2^-13 of
+    their largest products' sum; then one rounding to the result's type."""
+
+    m, n, k = shape
+    (a, sa), (b, sb) = (mdx.quantize_fp8(randn(96 + i, rows, k).abs()) for i, rows in enumerate((m, n)))
+    x, y = (c.double() * torch.exp2(s.contiguous().view(torch.uint8).double() - 127).repeat_interleave(128, 1)[:, :k]
+            for c, s in ((a, sa), (b, sb)))
+    want = x @ y.T.contiguous()
+    error = (2 * k + 16) * U * want
+    if dtype != torch.float32:
+        largest = [torch.nn.functional.pad(v, (0, -k % 8)).view(v.shape[0], -1, 8).amax(2) for v in (x, y)]
+        error = error + 7 * 2.0 ** -13 * (largest[0] @ largest[1].T.contiguous())
+    got = mdx.matmul_fp8(a, sa, b, sb, dtype=dtype).double()
+    assert torch.all(((want - error).to(dtype).double() <= got) & (got <= (want + error).to(dtype).double()))
