@@ -213,9 +213,11 @@ __global__ __launch_bounds__(Lanes > 256 ? Lanes : 256, 4) void k_norm_back(cons
     for (int64_t base = int64_t(blockIdx.x) * kRows; base < a.rows; base += int64_t(gridDim.x) * kRows) {
         // lanes without a row stay for the barrier and load zeros: another row's elements would not cancel (an infinite
         // gradient times a u of zero is NaN), and its owner may already store grad_x over them
-        const bool there = kRows == 1 || base + mine < a.rows;
+        // (one row a workgroup is always there; said as a constant, the kernels of 256 and more lanes spill: 20,000 x 7,380
+        // bfloat16 317 us, 215 so)
+        const bool there = base + mine < a.rows;
         const int64_t row = there ? base + mine : a.rows - 1;
-        const int here = there ? width : 0;
+        const int here = kRows == 1 || there ? width : 0;
         float t[Units][kUnit], h[Units][kUnit];
         const float rstd = there ? a.rstd[row] : 0.0f;
         float along = 0.0f;
