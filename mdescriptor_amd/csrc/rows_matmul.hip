@@ -122,94 +122,52 @@ __device__ __forceinline__ i8 load_block(const uint8_t* block, int quarter, int6
     return v;
 }
 
-// Rows of few: a workgroup of Waves wavefronts takes 16 MT x 16 NT outputs and
-// splits the blocks of 128 among them; their sums are joined through LDS in the
+// Rows of few: a workgroup of eight wavefronts takes 16 x 16 outputs and splits
+// the blocks of 128 among them; their sums are joined through LDS in the
 // wavefronts' order.  Operands go from memory straight to registers: nothing
-// is used twice.  Bound by b's bytes where they are many (1 x 4,096 x 7,380: 8.4
-// us, 3.6 TB/s) and by the few loads of each workgroup where they are not (1 x
+// is used twice.  Bound by b's bytes where they are many (1 x 4,096 x 7,380: 7.2
+// us, 4.2 TB/s) and by the few loads of each workgroup where they are not (1 x
 // 1,024 x 3,696: 4.8 us).  From 17 rows on tiles read b once for more of them (64
 // x 4,096 x 7,380: 12.5 us).
-template <typename O, int MT, int NT, int Waves>
-__global__ __launch_bounds__(Waves * kWave) void k_matmul_few(const MatmulView a, int64_t tiles_n, int64_t first) {
+constexpr int kFewWaves = 8;
+
+template <typename O>
+__global__ __launch_bounds__(kFewWaves * kWave) void k_matmul_few(const MatmulView a, int64_t tiles_n, int64_t first) {
     constexpr bool kExact = sizeof(O) == 4;
-    __shared__ f4 join[Waves > 1 ? Waves - 1 : 1][MT * NT][kWave];
+    __shared__ f4 join[kFewWaves - 1][kWave];
     const int lane = threadIdx.x % kWave, r = lane % 16, quarter = lane / 16;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int64_t at = first + int64_t(blockIdx.x), tile_m = at / tiles_n;
-    const int64_t m0 = tile_m * 16 * MT, n0 = (at - tile_m * tiles_n) * 16 * NT;
+    const int64_t m0 = tile_m * 16, n0 = (at - tile_m * tiles_n) * 16;
     const int64_t blocks = (a.k + kScaleBlock - 1) / kScaleBlock;
-    const uint8_t *rows_a[MT], *rows_b[NT], *scales_a[MT], *scales_b[NT];
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-        const int64_t row = min(m0 + 16 * i + r, a.m - 1);
-        rows_a[i] = a.a + row * a.a_pitch;
-        scales_a[i] = a.a_scales + row * a.a_scales_pitch;
-    }
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-        const int64_t row = min(n0 + 16 * j + r, a.n - 1);
-        rows_b[j] = a.b + row * a.b_pitch;
-        scales_b[j] = a.b_scales + (row >> a.b_shift) * a.b_scales_pitch;
-    }
-    f4 acc[MT][NT];
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < NT; ++j) acc[i][j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-    auto take = [&](const i8 (&ca)[MT], const i8 (&cb)[NT], const int (&sa)[MT], const int (&sb)[NT])
-        __attribute__((always_inline)) {
-        Fragment<kExact> fa[MT], fb[NT];
-#pragma unroll
-        for (int i = 0; i < MT; ++i) fa[i].set(ca[i], sa[i]);
-#pragma unroll
-        for (int j = 0; j < NT; ++j) fb[j].set(cb[j], sb[j]);
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int j = 0; j < NT; ++j) acc[i][j] = multiply(fa[i], fb[j], acc[i][j]);
-    };
-    for (int64_t block = wave; block < blocks; block += Waves) {
-        i8 ca[MT], cb[NT];
-        int sa[MT], sb[NT];
+    const int64_t row_a = min(m0 + r, a.m - 1), row_b = min(n0 + r, a.n - 1);
+    const uint8_t* codes_a = a.a + row_a * a.a_pitch;
+    const uint8_t* scales_a = a.a_scales + row_a * a.a_scales_pitch;
+    const uint8_t* codes_b = a.b + row_b * a.b_pitch;
+    const uint8_t* scales_b = a.b_scales + (row_b >> a.b_shift) * a.b_scales_pitch;
+    f4 acc{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int64_t block = wave; block < blocks; block += kFewWaves) {
         const int64_t left = a.k - block * kScaleBlock;
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            ca[i] = load_block(rows_a[i] + block * kScaleBlock, quarter, left);
-            sa[i] = scales_a[i][block];
-        }
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            cb[j] = load_block(rows_b[j] + block * kScaleBlock, quarter, left);
-            sb[j] = scales_b[j][block];
-        }
-        take(ca, cb, sa, sb);
+        const i8 ca = load_block(codes_a + block * kScaleBlock, quarter, left);
+        const int sa = scales_a[block];
+        const i8 cb = load_block(codes_b + block * kScaleBlock, quarter, left);
+        const int sb = scales_b[block];
+        Fragment<kExact> fa, fb;
+        fa.set(ca, sa);
+        fb.set(cb, sb);
+        acc = multiply(fa, fb, acc);
     }
-    if constexpr (Waves > 1) {
-        if (wave > 0) {
+    if (wave > 0) join[wave - 1][lane] = acc;
+    __syncthreads();
+    if (wave > 0) return;
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int j = 0; j < NT; ++j) join[wave - 1][i * NT + j][lane] = acc[i][j];
-        }
-        __syncthreads();
-        if (wave > 0) return;
-#pragma unroll
-        for (int w = 0; w < Waves - 1; ++w)
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int j = 0; j < NT; ++j) acc[i][j] += join[w][i * NT + j][lane];
-    }
+    for (int w = 0; w < kFewWaves - 1; ++w) acc += join[w][lane];
     O* out = static_cast<O*>(a.out);
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                const int64_t row = m0 + 16 * i + 4 * quarter + v, col = n0 + 16 * j + r;
-                if (row < a.m && col < a.n) out[row * a.out_pitch + col] = static_cast<O>(acc[i][j][v]);
-            }
+    for (int v = 0; v < 4; ++v) {
+        const int64_t row = m0 + 4 * quarter + v, col = n0 + r;
+        if (row < a.m && col < a.n) out[row * a.out_pitch + col] = static_cast<O>(acc[v]);
+    }
 }
 
 // s_waitcnt's operand for at most n loads under way and no reads of LDS.
@@ -722,8 +680,8 @@ template <typename O> void run_matmul(const MatmulView& v, const MatmulPlan& pla
     constexpr bool kExact = sizeof(O) == 4;
     if (plan.tile < 0) {
         const int64_t tiles_n = (v.n + 15) / 16, tiles_m = (v.m + 15) / 16;
-        in_runs(tiles_m * tiles_n, 512, [&](int64_t first, int64_t count) {
-            k_matmul_few<O, 1, 1, 8><<<dim3(unsigned(count)), 512, 0, s>>>(v, tiles_n, first);
+        in_runs(tiles_m * tiles_n, kFewWaves * kWave, [&](int64_t first, int64_t count) {
+            k_matmul_few<O><<<dim3(unsigned(count)), kFewWaves * kWave, 0, s>>>(v, tiles_n, first);
             MDX_HIP(hipGetLastError());
         });
     } else if (plan.slices == 1) {
