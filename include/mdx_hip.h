@@ -367,7 +367,8 @@ enum { MDX_FLOAT32 = 0, MDX_BFLOAT16 = 1, MDX_FLOAT16 = 2, MDX_FLOAT8 = 3 };
  * in float32 and rounded once to out_dtype (dtype's own, or MDX_FLOAT8 with
  * scales[rows, blocks of 128]).  residual (may be NULL) has x's dtype; with
  * it, total (may be NULL) receives t rounded to dtype.  rstd (may be NULL):
- * f32[rows].  gain: f32[width].  total may be x or residual itself. */
+ * f32[rows].  gain: f32[width].  total may be x or residual itself.  A row
+ * whose sum of squares passes float32's range has rstd zero. */
 typedef struct mdx_norm_args {
     int64_t rows, width;
     const void* x;

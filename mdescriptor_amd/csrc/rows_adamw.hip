@@ -5,8 +5,8 @@
 // by HBM, or by the launch where the tensors are small.  The tensors' pointers
 // travel in the kernel's arguments: nothing is copied to the device ahead of
 // the launch, nothing is kept from step to step, and 48 tensors take one
-// launch.  40 tensors of 60.6 M elements with 8-bit states take 155 us (5.4
-// TB/s), twelve of 0.9 M with 32-bit states 6 us.
+// launch.  40 tensors of 60.4 M elements with 8-bit states take 154 us (5.5
+// TB/s), twelve of 0.56 M with 32-bit states 5.8 us.
 #include "rows_device.h"
 
 #include <algorithm>
@@ -21,7 +21,7 @@ using namespace rows;
 
 typedef uint32_t u2_any __attribute__((ext_vector_type(2), aligned(1))); // eight codes at any address
 
-constexpr int kTensors = 48;            // per launch: 48 * 72 bytes of arguments, under the 4 KB of a launch
+constexpr int kTensors = 48;            // per launch: 48 * 68 bytes of arguments and the numbers, under the 4 KB of a launch
 constexpr int kChunk = 256 * kUnit;    // elements per workgroup: with two or four units a lane, 5 and 20 % slower
 static_assert(kChunk == kAdamwChunk, "the size that the entry point refuses follows from it");
 
@@ -101,7 +101,7 @@ __device__ __forceinline__ u2 load_codes(const uint8_t* codes, int64_t at, int64
 }
 
 // Moving: step and seed, as far as they are given so, come from device memory (0.3 us more for twelve tensors, 158 us in
-// place of 154 for 60.5 M elements with 8-bit states: the corrections are computed by every wavefront).
+// place of 154 for 60.4 M elements with 8-bit states: the corrections are computed by every wavefront).
 template <typename G, bool Codes, bool Moving> __global__ __launch_bounds__(256) void k_adamw(const AdamwTable a) {
     const int64_t chunk = blockIdx.x;
     uint32_t seed = a.seed;
@@ -155,7 +155,7 @@ template <typename G, bool Codes, bool Moving> __global__ __launch_bounds__(256)
         v[i] = fmaf(a.beta2, v[i], a.rest2 * g[i] * g[i]);
         // the device's own root and reciprocal, good to one unit in the last place (a v below the normal numbers has
         // the root zero); correctly rounded ones take ten instructions each, and the 8-bit step is then bound by
-        // them: 195 us in place of 161 for 60.5 M elements
+        // them: 195 us in place of 161 for 60.4 M elements
         r[i] = __builtin_amdgcn_sqrtf(v[i]);
         p[i] = fmaf(p[i], a.keep, -(rate * m[i]) * __builtin_amdgcn_rcpf(fmaf(r[i], root, a.eps)));
     }

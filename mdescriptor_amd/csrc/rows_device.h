@@ -65,7 +65,7 @@ __device__ __forceinline__ void load_unit(const T* row, I col, I width, float (&
 // The same for rows whose lanes wait for each other: the end of a row, n < 8
 // elements, in accesses of four, two and one that are under way together,
 // where up to seven conditional ones follow each other (gradients of 20,000 x
-// 7,380 bfloat16 276 us, 330 with those).  The norm itself gains nothing by it
+// 7,380 bfloat16 with a residual's 276 us, 330 with those).  The norm itself gains nothing by it
 // (65,536 x 3,696 bfloat16 165 us, 157 without).
 template <typename T> __device__ __forceinline__ void load_unit_together(const T* row, int col, int width, float (&v)[kUnit]) {
     if (col + kUnit <= width) {

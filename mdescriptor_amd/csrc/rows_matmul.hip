@@ -212,10 +212,12 @@ __device__ __forceinline__ i8 cut(i8 v, int left) {
 // gridDim.y > 1 splits the contraction: slice y takes 64 stages_per of it from
 // y * 64 stages_per on and stores float32 sums to its own matrix of the workspace.
 //
-// Measured: 65,536 x 1,024 x 3,696 to bfloat16 208-217 us (2.3 PFLOP/s), 8,192
-// cubed 394 us (2.8 PFLOP/s; all codes zero: 293 us, 3.75).  Random operands
-// are bound by power, at 1.4 to 1.8 GHz: the matrix cores are busy for two thirds
-// of the cycles.  To float32: 8,192 cubed 815 us (1.35 PFLOP/s; zeros 620), the
+// Measured: 65,536 x 1,024 x 3,696 to bfloat16 193 us call upon call (2.6
+// PFLOP/s), 8,192 cubed 383 us (2.9 PFLOP/s; all codes zero: 293 us, 3.75).
+// Random operands are bound by power, at 1.4 to 1.8 GHz: the matrix cores are
+// busy for two thirds of the cycles.  After a pause the first calls of the
+// former take 200 us, those from 2 to 5 ms on up to 270, while the clock is
+// brought down and settles.  To float32: 8,192 cubed 815 us (1.35 PFLOP/s; zeros 620), the
 // rate of bfloat16 products of that size.
 template <typename O, bool Exact, int TM, int TN, int WR, int WC, int Halves, int Buffers>
 __global__ __launch_bounds__(WR * WC * kWave) void k_matmul_tile(const MatmulView a, int tiles_m, int tiles_n,

@@ -5,7 +5,7 @@
 // A row is read once: its units stay in registers between the sum of squares
 // and the products, so both directions move each byte once and are bound by
 // HBM once there are rows enough to fill the device: 65,536 x 3,696 float32 to
-// float8 takes 217 us (5.6 TB/s), the gradients of 65,536 x 1,024 bfloat16 with a
+// float8 takes 210 us (5.8 TB/s), the gradients of 65,536 x 1,024 bfloat16 with a
 // residual's 100 us (5.35 TB/s).  One row of 3,696 takes 2.8 us on the device.
 #include "rows_device.h"
 
@@ -214,7 +214,7 @@ __global__ __launch_bounds__(Lanes > 256 ? Lanes : 256, 4) void k_norm_back(cons
         // lanes without a row stay for the barrier and load zeros: another row's elements would not cancel (an infinite
         // gradient times a u of zero is NaN), and its owner may already store grad_x over them
         // (one row a workgroup is always there; said as a constant, the kernels of 256 and more lanes spill: 20,000 x 7,380
-        // bfloat16 317 us, 215 so)
+        // bfloat16 without a residual's gradient 317 us, 215 so)
         const bool there = base + mine < a.rows;
         const int64_t row = there ? base + mine : a.rows - 1;
         const int here = kRows == 1 || there ? width : 0;
@@ -373,7 +373,7 @@ struct BackShape {
 
 // Lanes per row, units per lane and workgroups: no more than there are rows
 // for, and than the device holds at once, so that the partial rows are few
-// (5,321 x 5,621 float32: 85 us, 107 with twice the workgroups).
+// (5,321 x 5,621 float32 without a residual's: 84 us, 107 with twice the workgroups).
 BackShape back_shape(int64_t rows, int64_t width) {
     BackShape b{1024, 0, 1};
     // two units a lane: 128 registers, four wavefronts a SIMD.  One unit and twice the lanes is 5 % slower at 1,024 to

@@ -117,7 +117,8 @@ def rms_norm(rows: torch.Tensor, gain: torch.Tensor, *, residual: torch.Tensor |
     type, ``gain`` a float32 vector.  ``dtype`` is the rows' own type (the
     default) or ``torch.float8_e4m3fn``, which gives scales too.  Everything
     is computed in float32 and rounded once.  A NaN makes its whole row NaN; an
-    infinity makes its element NaN and the rest of the row zero."""
+    infinity makes its element NaN and the rest of the row zero; a row whose sum
+    of squares passes float32's range (elements about 2**64 and larger) is zero."""
 
     return NormResult._make(_calls.rms_norm(rows, gain, residual, eps, dtype))
 

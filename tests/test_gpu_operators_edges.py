@@ -534,3 +534,16 @@ def test_product_of_equal_signs(dtype, shape):
         error = error + 7 * 2.0 ** -13 * (largest[0] @ largest[1].T.contiguous())
     got = mdx.matmul_fp8(a, sa, b, sb, dtype=dtype).double()
     assert torch.all(((want - error).to(dtype).double() <= got) & (got <= (want + error).to(dtype).double()))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_norm_of_rows_whose_squares_pass_the_range(dtype):
+    """2^64 squared is past float32: rstd and the row are zero, the rows beside it are not touched."""
+
+    x, gain = randn(100, 6, 200, dtype=dtype), randn(101, 200)
+    want = mdx.rms_norm(x, gain)
+    x[2, 7] = 2.0 ** 64
+    got = mdx.rms_norm(x, gain)
+    assert float(got.rstd[2]) == 0.0 and not got.values[2].any()
+    rest = torch.arange(6, device="cuda") != 2
+    assert torch.equal(got.values[rest], want.values[rest]) and torch.equal(got.rstd[rest], want.rstd[rest])
