@@ -341,11 +341,12 @@ void mdx_hip_host_free(void* ptr);
  * All pointers inside the argument structs are device pointers of `device`;
  * the structs themselves are host memory and are read before the call
  * returns.  Each call only queues kernels on `stream` (a hipStream_t; NULL is
- * the default stream) and allocates nothing, so it can be captured into a
- * graph (whose replays repeat its numbers: see mdx_adamw_args), and calls on different streams do not wait for each other.  Calls
- * keep nothing: a workspace is the caller's and is free again when the
- * stream has passed the call.  A workspace of sizes that the call refuses has
- * zero bytes.  Errors: mdx_hip_last_error(NULL), per thread.
+ * the default stream) and allocates nothing on the device, so it can be
+ * captured into a graph (whose replays repeat its numbers: see
+ * mdx_hip_adamw_step_at) and calls on different streams do not wait for each
+ * other.  Calls keep nothing: a workspace is the caller's and is free again
+ * when the stream has passed the call.  A workspace of sizes that the call
+ * refuses has zero bytes.  Errors: mdx_hip_last_error(NULL), per thread.
  *
  * Matrices are row-major with a pitch in elements; any pitch >= width and any
  * alignment to the element's own size is taken, 16-byte aligned rows are the
@@ -493,10 +494,7 @@ int mdx_hip_matmul_fp8(int device, const mdx_matmul_args* args, void* stream);
  *
  * A graph that has captured the call repeats its numbers on every replay: the
  * same step, the same bias corrections and the same random bits, by which v
- * would stand still after all.  step_at and seed_at (each may be NULL) are
- * device addresses of numbers that are read in place of step and seed when the
- * kernels run (of the seed the low 32 bits), so that a replay goes on with what the
- * graph or its caller has written there.  A step below 1 there changes nothing. */
+ * would stand still after all.  mdx_hip_adamw_step_at is the call for graphs. */
 typedef struct mdx_adamw_tensor {
     int64_t n;
     float* params;
@@ -514,10 +512,16 @@ typedef struct mdx_adamw_args {
     uint32_t seed;
     int32_t grad_dtype;
     int32_t bits;
-    const int64_t* step_at;
-    const int64_t* seed_at;
 } mdx_adamw_args;
 int mdx_hip_adamw_step(int device, const mdx_adamw_args* args, void* stream);
+
+/* The same with numbers from device memory: step_at and seed_at (each may be
+ * NULL) are device addresses of numbers that are read in place of args->step
+ * and args->seed when the kernels run (of the seed the low 32 bits), so that a
+ * replay goes on with what the graph or its caller has written there.  A step
+ * below 1 there changes nothing. */
+int mdx_hip_adamw_step_at(int device, const mdx_adamw_args* args, const int64_t* step_at, const int64_t* seed_at,
+                          void* stream);
 
 /* Library version and build target, for diagnostics. */
 const char* mdx_hip_version(void);

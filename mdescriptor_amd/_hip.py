@@ -302,8 +302,6 @@ class AdamwArgs(ctypes.Structure):
         ("seed", ctypes.c_uint32),
         ("grad_dtype", ctypes.c_int32),
         ("bits", ctypes.c_int32),
-        ("step_at", ctypes.c_void_p),
-        ("seed_at", ctypes.c_void_p),
     ]
 
 
@@ -371,6 +369,8 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     "mdx_hip_matmul_fp8_workspace": (ctypes.c_int64, [ctypes.POINTER(MatmulArgs)]),
     "mdx_hip_matmul_fp8": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(MatmulArgs), ctypes.c_void_p]),
     "mdx_hip_adamw_step": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(AdamwArgs), ctypes.c_void_p]),
+    "mdx_hip_adamw_step_at": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(AdamwArgs), ctypes.c_void_p, ctypes.c_void_p,
+                                             ctypes.c_void_p]),
     "mdx_hip_version": (ctypes.c_char_p, []),
 }
 

@@ -189,7 +189,7 @@ template <typename G> void launch_adamw(const AdamwTable& t, bool codes, hipStre
 
 } // namespace
 
-void adamw_step(const mdx_adamw_args& g, hipStream_t s) {
+void adamw_step(const mdx_adamw_args& g, const int64_t* step_at, const int64_t* seed_at, hipStream_t s) {
     AdamwTable t{};
     const double step = double(g.step);
     t.keep = float(1.0 - g.lr * g.weight_decay);
@@ -201,8 +201,8 @@ void adamw_step(const mdx_adamw_args& g, hipStream_t s) {
     t.rest1 = float(1.0 - g.beta1);
     t.rest2 = float(1.0 - g.beta2);
     t.seed = g.seed;
-    t.step_at = g.step_at;
-    t.seed_at = g.seed_at;
+    t.step_at = step_at;
+    t.seed_at = seed_at;
     t.lr = g.lr;
     t.log1 = std::log(g.beta1);
     t.log2 = std::log(g.beta2);

@@ -212,6 +212,11 @@ int mdx_hip_matmul_fp8(int device, const mdx_matmul_args* args, void* stream) {
 }
 
 int mdx_hip_adamw_step(int device, const mdx_adamw_args* args, void* stream) {
+    return mdx_hip_adamw_step_at(device, args, nullptr, nullptr, stream);
+}
+
+int mdx_hip_adamw_step_at(int device, const mdx_adamw_args* args, const int64_t* step_at, const int64_t* seed_at,
+                          void* stream) {
     return mdx::guarded_call([&] {
         require(args != nullptr, "arguments must not be null");
         const mdx_adamw_args& g = *args;
@@ -219,8 +224,8 @@ int mdx_hip_adamw_step(int device, const mdx_adamw_args* args, void* stream) {
         require(g.bits == 8 || g.bits == 32, "states have 8 or 32 bits");
         require(g.count >= 0 && g.count < kMostRows && (g.count == 0 || g.tensors != nullptr),
                 "the tensors must not be null");
-        require(g.step_at != nullptr || g.step >= 1, "step must be at least 1");
-        require(reinterpret_cast<uintptr_t>(g.step_at) % 8 == 0 && reinterpret_cast<uintptr_t>(g.seed_at) % 8 == 0,
+        require(step_at != nullptr || g.step >= 1, "step must be at least 1");
+        require(reinterpret_cast<uintptr_t>(step_at) % 8 == 0 && reinterpret_cast<uintptr_t>(seed_at) % 8 == 0,
                 "step_at and seed_at must be aligned to their numbers");
         require(std::isfinite(g.lr) && g.lr >= 0.0, "lr must be finite and not negative");
         require(g.beta1 >= 0.0 && g.beta1 < 1.0 && g.beta2 >= 0.0 && g.beta2 < 1.0, "betas must lie in [0, 1)");
@@ -240,7 +245,7 @@ int mdx_hip_adamw_step(int device, const mdx_adamw_args* args, void* stream) {
         }
         check_apart(g);
         OnDevice on(device);
-        mdx::adamw_step(g, static_cast<hipStream_t>(stream));
+        mdx::adamw_step(g, step_at, seed_at, static_cast<hipStream_t>(stream));
     });
 }
 

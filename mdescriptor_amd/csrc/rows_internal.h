@@ -28,7 +28,7 @@ void rms_norm_backward(const mdx_norm_backward_args& args, hipStream_t stream);
 void quantize_fp8(const mdx_quantize_args& args, hipStream_t stream);
 int64_t matmul_fp8_workspace(const mdx_matmul_args& args);
 void matmul_fp8(const mdx_matmul_args& args, hipStream_t stream);
-void adamw_step(const mdx_adamw_args& args, hipStream_t stream);
+void adamw_step(const mdx_adamw_args& args, const int64_t* step_at, const int64_t* seed_at, hipStream_t stream);
 
 // Calls run() and turns what it throws into a status and this thread's last error.
 int guarded_call(const std::function<void()>& run);

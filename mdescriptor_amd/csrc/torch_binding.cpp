@@ -553,8 +553,8 @@ PyObject* adamw_step(PyObject*, PyObject* const* o, Py_ssize_t n) {
         const at::Tensor& lead = given[0]->at(0);
         if (!lead.is_cuda()) throw Refused{"params must live on a HIP device", "params"};
         const at::Device device = lead.device();
-        if (moving_step) a.step_at = number_at(o[6], "step", device);
-        if (moving_seed) a.seed_at = number_at(o[12], "seed", device);
+        const int64_t* step_at = moving_step ? number_at(o[6], "step", device) : nullptr;
+        const int64_t* seed_at = moving_seed ? number_at(o[12], "seed", device) : nullptr;
         const at::ScalarType grad_type = given[1]->at(0).scalar_type();
         if (kind_of(grad_type) < 0) throw Refused{"grads must be float32, bfloat16 or float16 tensors", "grads"};
         a.grad_dtype = kind_of(grad_type);
@@ -586,7 +586,7 @@ PyObject* adamw_step(PyObject*, PyObject* const* o, Py_ssize_t n) {
         a.tensors = table.data();
         a.count = count;
         void* stream = stream_of(device);
-        run("adamw_step", [&] { return mdx_hip_adamw_step(device.index(), &a, stream); });
+        run("adamw_step", [&] { return mdx_hip_adamw_step_at(device.index(), &a, step_at, seed_at, stream); });
         for (int i = 0; i < lists; ++i)
             for (Py_ssize_t k = 0; i != 1 && k < count; ++k) written_to(given[i]->at(k));
         return none();

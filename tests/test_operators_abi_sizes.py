@@ -75,11 +75,17 @@ def test_adamw_takes_a_step_from_device_memory_in_place_of_the_number(hip):
     lib = hip.load_library()
     values = dict(tensors=None, count=0, lr=1e-3, beta1=0.9, beta2=0.99, eps=1e-8, weight_decay=0.0, step=0, seed=0,
                   grad_dtype=0, bits=32)
-    call = lambda **c: lib.mdx_hip_adamw_step(0, ctypes.byref(hip.AdamwArgs(**{**values, **c})), None)  # noqa: E731
-    assert call() == hip.MDX_INVALID_ARGUMENT and "step must" in lib.mdx_hip_last_error(None).decode()
-    for name in ("step_at", "seed_at"):
-        assert call(**{"step": 1, name: P + 4}) == hip.MDX_INVALID_ARGUMENT
-        assert "aligned" in lib.mdx_hip_last_error(None).decode()
+
+    def call(step, step_at, seed_at):
+        args = hip.AdamwArgs(**{**values, "step": step})
+        return lib.mdx_hip_adamw_step_at(0, ctypes.byref(args), step_at, seed_at, None), lib.mdx_hip_last_error(None).decode()
+
+    status, message = call(0, None, None)
+    assert status == hip.MDX_INVALID_ARGUMENT and "step must" in message
+    for places in ((P + 4, None), (None, P + 4)):
+        status, message = call(1, *places)
+        assert status == hip.MDX_INVALID_ARGUMENT and "aligned" in message
+    assert lib.mdx_hip_adamw_step_at(0, None, None, None, None) == hip.MDX_INVALID_ARGUMENT
 
 
 M = 1 << 20  # addresses far apart that nothing here reads
